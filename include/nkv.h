@@ -56,6 +56,7 @@ typedef enum nkv_status {
 #define NKV_DEVERR_PREFILL_RANGE   0x20u /* cu_seqlens / max_seqlen_q outside the tensors or the grid */
 #define NKV_DEVERR_ROPE_POSITION   0x40u /* position outside the rotary cos/sin cache (clamped) */
 #define NKV_DEVERR_LAUNCH_SHAPE    0x80u /* a kernel ran without the thread-block clusters it needs (nothing written) */
+#define NKV_DEVERR_PAGES           0x100u /* page operators: a row or page out of range, named twice or both read and written, a page already free, or no free page left */
 
 /* Human-readable name of a status code (static string). */
 const char* nkv_status_string(int status);
@@ -416,6 +417,141 @@ int nkv_paged_decode_static_scratch(const void* q, int64_t q_stride_token, int64
                                     int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                     int32_t head_dim, int32_t block_size, float softmax_scale,
                                     void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* 5. 8-bit KV cache                                                         */
+/* No counterpart in the reference, whose cache is bf16: an addition that    */
+/* halves the bytes of a cached token. A row (one token, one kv head, K or   */
+/* V) is held as head_dim e4m3 values and one exponent byte and stands for   */
+/* e4m3 * 2^(byte - 127). Values: [num_blocks, block_size, Hk, 128], one     */
+/* byte each, addressed by slots like the bf16 cache; exponent bytes:        */
+/* [num_blocks, Hk, block_size]. Supported by every call of this section:    */
+/* head_dim 128; block_size 16, 32, 64 or a multiple of 128; num_blocks *    */
+/* block_size < 2^31; 16-byte aligned caches and exponent bytes.             */
+
+/* Quantised slot write. Row x of token i and kv head h goes to slot         */
+/* s = slot_mapping[i] (-1: skipped; other slots outside the cache are not   */
+/* written and flag NKV_DEVERR_STORE_SLOT): with a the largest finite |x_j|  */
+/* and k the smallest integer with a <= 448 * 2^k, kept in [-117, 119]       */
+/* (a == 0: -117), byte = k + 127 and value_j = e4m3(x_j * 2^-k) rounded to  */
+/* nearest even; an infinity becomes +-448, a NaN stays one. key / value     */
+/* rows as nkv_store_kvcache (strides in elements, multiples of 8).          */
+int nkv_store_kvcache_fp8(const void* key, int64_t key_stride, const void* value,
+                          int64_t value_stride, void* k_cache, void* v_cache, void* k_exp,
+                          void* v_exp, int64_t num_blocks, int32_t block_size,
+                          const int32_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
+                          int32_t head_dim, void* stream);
+
+/* Read-back of whole sequences as bf16 rows (exact: every stored value is a */
+/* bf16 number): row cu_seqlens[b] + j of k_out / v_out ([num_tokens, Hk,    */
+/* 128], row strides in elements) gets position j of sequence b, found       */
+/* through block_tables [batch, max_blocks]. Rows outside [cu_seqlens[0],    */
+/* cu_seqlens[batch]) are left as they are. A position past the block table  */
+/* is left as it is and flags NKV_DEVERR_PREFILL_RANGE; one whose table      */
+/* entry is no page reads as zeros and flags NKV_DEVERR_DECODE_BLOCK. What   */
+/* nkv_paged_prefill takes for a prompt whose prefix is cached in 8 bits.    */
+int nkv_load_kvcache_fp8(const void* k_cache, const void* v_cache, const void* k_exp,
+                         const void* v_exp, int64_t num_blocks, int32_t block_size,
+                         const int32_t* block_tables, int32_t max_blocks,
+                         const int32_t* cu_seqlens, int32_t batch, int64_t num_tokens, void* k_out,
+                         int64_t k_out_stride, void* v_out, int64_t v_out_stride,
+                         int32_t num_kv_heads, int32_t head_dim, void* stream);
+
+/* nkv_paged_decode over the 8-bit cache: same arguments and result (keys    */
+/* and values are what the stored rows stand for; a length 0 writes zeros; a */
+/* length past the block table is clamped and flags                          */
+/* NKV_DEVERR_DECODE_BLOCK, as does an entry on a live token that is no      */
+/* page). g = num_q_heads / num_kv_heads in [1, 16]; batch * num_kv_heads    */
+/* <= 65536; q and out 16-byte aligned, strides multiples of 8. The          */
+/* workspace needs no particular content and nothing in it outlives the      */
+/* call: calls that may overlap on the GPU take one each.                    */
+size_t nkv_paged_decode_fp8_workspace_size(int32_t num_q_heads, int32_t num_kv_heads);
+int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride_head,
+                         const void* k_cache, const void* v_cache, const void* k_exp,
+                         const void* v_exp, int64_t num_blocks, const int32_t* block_tables,
+                         int32_t max_blocks, const int32_t* context_lens, void* out,
+                         int64_t out_stride_token, int32_t batch, int32_t num_q_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                         float softmax_scale, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* 6. Pages of a cache                                                       */
+/* No counterpart in the reference, whose host BlockManager hands pages out  */
+/* and never moves or shares a partly filled one. Device-side state, all     */
+/* int32: block_tables [num_rows, max_blocks] (-1 = no page), context_lens   */
+/* [num_rows], ref_counts [num_pages] (table entries that name the page;     */
+/* <= 0 = free). Every decision is taken on the device, so the calls can be  */
+/* captured in a CUDA graph; free pages are taken lowest first. Tables and   */
+/* counts named by a call must not be changed by another one that may        */
+/* overlap with it.                                                          */
+
+/* One cache tensor (host struct): `lead` copies (layers, K and V) of        */
+/* num_pages contiguous pages, lead_stride bytes apart. A page is page_bytes */
+/* long and consists of segments of seg_bytes = block_size * token_bytes     */
+/* bytes each (one for bf16 or 8-bit values: token_bytes = Hk * 128 * size;  */
+/* Hk for exponent bytes: token_bytes = 1), so n tokens of a page are the    */
+/* first n * token_bytes bytes of each segment. base 16-byte aligned,        */
+/* lead_stride and seg_bytes multiples of 16. At most 256 regions per call.  */
+typedef struct nkv_page_region {
+  void* base;
+  int64_t lead;
+  int64_t lead_stride;
+  int64_t page_bytes;
+  int64_t seg_bytes;
+  int64_t token_bytes;
+} nkv_page_region;
+
+/* Workspace of the three calls that take one, for n pairs or forks (copy,   */
+/* fork: num_pages 0; compact: n = num_pages / 2). Needs no particular       */
+/* content; calls that may overlap on the GPU take one each.                 */
+size_t nkv_pages_workspace_size(int64_t n, int64_t num_pages);
+
+/* Copies page src[i] to page dst[i] in every region. A page may be read by  */
+/* several pairs; a pair whose target another pair writes or any pair reads, */
+/* or with a page outside the cache, is not copied and flags                 */
+/* NKV_DEVERR_PAGES. (-1, -1) pairs are padding.                             */
+int nkv_copy_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
+                   const int32_t* src, const int32_t* dst, int32_t n, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* Row dst_rows[i] becomes a copy of row src_rows[i]: the pages dst_rows[i]  */
+/* holds lose a reference (all of them before any page is handed out); the   */
+/* full pages of the source are shared (a reference more); a partial last    */
+/* page is copied -- its first context_lens % block_size tokens, in every    */
+/* region -- to the lowest free page (the i-th fork that wants one, in       */
+/* order, gets the i-th lowest); context_lens[dst] = context_lens[src], the  */
+/* table's other entries -1. out_pages[i] = that page, -1 if none was        */
+/* needed, -2 if the fork was not made: a row outside the table, a target    */
+/* named twice or also a source (nothing changes), or no free page (the      */
+/* target is left empty); each flags NKV_DEVERR_PAGES. A source may be named */
+/* by several forks. (-1, -1) pairs are padding (out_pages -2, no flag).     */
+int nkv_fork_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
+                   int32_t block_size, int32_t* block_tables, int32_t max_blocks, int32_t num_rows,
+                   int32_t* context_lens, int32_t* ref_counts, const int32_t* src_rows,
+                   const int32_t* dst_rows, int32_t n, int32_t* out_pages, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* Rows rows[i] (-1: padding) give up their pages: each loses a reference    */
+/* and its table entry becomes -1. trim = 0: all of them, context_lens = 0;  */
+/* trim = 1: those past context_lens, which stays (after a compression has   */
+/* shortened the rows on the device). A row named twice loses its pages      */
+/* once; a page that was already free flags NKV_DEVERR_PAGES.                */
+int nkv_free_pages(int32_t* block_tables, int32_t max_blocks, int32_t num_rows,
+                   int32_t* context_lens, int32_t* ref_counts, int64_t num_pages,
+                   int32_t block_size, const int32_t* rows, int32_t n, int32_t trim,
+                   void* stream);
+
+/* Brings the n pages in use to [0, n): the i-th page in use at or past n    */
+/* moves to the i-th free page before n (both counted upwards) in every      */
+/* region, counts and the num_entries table entries follow. Out of place for */
+/* tables and counts unless the out pointers are the same; out_num_live gets */
+/* n. An entry that names a free page or none of the cache stays as it is    */
+/* and flags NKV_DEVERR_PAGES.                                               */
+int nkv_compact_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
+                      const int32_t* block_tables, int32_t* out_block_tables, int64_t num_entries,
+                      const int32_t* ref_counts, int32_t* out_ref_counts, int32_t* out_num_live,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -12,8 +12,11 @@
 #include <cstring>
 #include <mutex>
 
+#include "cache_pages.cuh"
+#include "fp8_cache.cuh"
 #include "nkv_common.cuh"
 #include "paged_decode.cuh"
+#include "paged_decode_fp8.cuh"
 #include "paged_prefill.cuh"
 #include "qk_norm_rope.cuh"
 #include "oproj_allreduce.cuh"
@@ -1259,3 +1262,435 @@ extern "C" int nkv_paged_decode_static_scratch(
                           num_q_heads, num_kv_heads, head_dim, block_size, softmax_scale, scratch,
                           NKV_STATIC_SCRATCH_BYTES, stream);
 }
+
+// ---------------------------------------------------------------- 8-bit cache
+namespace {
+
+// Launch that may start while its predecessor in the stream drains; the kernel
+// waits (griddepcontrol.wait) before it touches global memory.
+template <typename... KArgs, typename... Args>
+int launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                     cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+// Pages of 16, 32, 64 or a multiple of 128 tokens: a 128-token decode tile is
+// then a whole number of pages or lies inside one.
+bool page8_size_ok(int block_size) {
+  return block_size == 16 || block_size == 32 || block_size == 64 ||
+         (block_size > 0 && block_size % 128 == 0);
+}
+
+// Arguments every 8-bit cache call shares.
+int check_cache8(const void* k_cache, const void* v_cache, const void* k_exp, const void* v_exp,
+                 int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim) {
+  if (num_blocks < 0 || num_kv_heads <= 0 || block_size <= 0 || head_dim <= 0)
+    return NKV_ERR_INVALID_ARGUMENT;
+  if (head_dim != 128 || !page8_size_ok(block_size)) return NKV_ERR_UNSUPPORTED;
+  if (num_blocks * block_size > 0x7fffffff) return NKV_ERR_UNSUPPORTED;  // slots are int32
+  if (!k_cache || !v_cache || !k_exp || !v_exp) return NKV_ERR_INVALID_ARGUMENT;
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_exp) || !aligned16(v_exp))
+    return NKV_ERR_ALIGNMENT;
+  return NKV_OK;
+}
+
+int launch_rows8(void (*kernel)(nkv::Rows8Params), const nkv::Rows8Params& p, void* stream) {
+  const int64_t per_block = static_cast<int64_t>(nkv::kRows8Warps) * nkv::kRows8PerWarp;
+  const int64_t blocks = (p.num_rows + per_block - 1) / per_block;
+  if (blocks > 0x7fffffff) return NKV_ERR_UNSUPPORTED;
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), dim3(nkv::kRows8Warps * 32),
+                          0, static_cast<cudaStream_t>(stream), p);
+}
+
+template <int G>
+int launch_decode8(const nkv::Decode8Params& p, void* stream) {
+  return launch_dependent(nkv::paged_decode_fp8_kernel<G>, dim3(p.batch * p.num_kv_heads),
+                          dim3(nkv::kDecode8Warps * 32), 0, static_cast<cudaStream_t>(stream), p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int nkv_store_kvcache_fp8(const void* key, int64_t key_stride, const void* value,
+                          int64_t value_stride, void* k_cache, void* v_cache, void* k_exp,
+                          void* v_exp, int64_t num_blocks, int32_t block_size,
+                          const int32_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
+                          int32_t head_dim, void* stream) {
+  if (num_tokens < 0) return NKV_ERR_INVALID_ARGUMENT;
+  if (num_tokens == 0 || num_blocks == 0) return NKV_OK;
+  const int st = check_cache8(k_cache, v_cache, k_exp, v_exp, num_blocks, block_size, num_kv_heads,
+                              head_dim);
+  if (st != NKV_OK) return st;
+  if (!key || !value || !slot_mapping) return NKV_ERR_INVALID_ARGUMENT;
+  const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (key_stride < row || value_stride < row) return NKV_ERR_INVALID_ARGUMENT;
+  if ((key_stride % 8) != 0 || (value_stride % 8) != 0 || !aligned16(key) || !aligned16(value))
+    return NKV_ERR_ALIGNMENT;
+  nkv::Rows8Params p{};
+  p.cache[0] = static_cast<uint8_t*>(k_cache);
+  p.cache[1] = static_cast<uint8_t*>(v_cache);
+  p.exps[0] = static_cast<uint8_t*>(k_exp);
+  p.exps[1] = static_cast<uint8_t*>(v_exp);
+  p.num_blocks = num_blocks;
+  p.num_kv_heads = num_kv_heads;
+  p.block_size = block_size;
+  p.src[0] = static_cast<const __nv_bfloat16*>(key);
+  p.src[1] = static_cast<const __nv_bfloat16*>(value);
+  p.src_stride[0] = key_stride;
+  p.src_stride[1] = value_stride;
+  p.slot_mapping = slot_mapping;
+  p.num_rows = static_cast<int64_t>(num_tokens) * 2 * num_kv_heads;
+  return launch_rows8(nkv::store_kvcache_fp8_kernel, p, stream);
+}
+
+int nkv_load_kvcache_fp8(const void* k_cache, const void* v_cache, const void* k_exp,
+                         const void* v_exp, int64_t num_blocks, int32_t block_size,
+                         const int32_t* block_tables, int32_t max_blocks,
+                         const int32_t* cu_seqlens, int32_t batch, int64_t num_tokens, void* k_out,
+                         int64_t k_out_stride, void* v_out, int64_t v_out_stride,
+                         int32_t num_kv_heads, int32_t head_dim, void* stream) {
+  if (num_tokens < 0 || batch < 0 || max_blocks < 0) return NKV_ERR_INVALID_ARGUMENT;
+  if (num_tokens == 0 || batch == 0) return NKV_OK;
+  const int st = check_cache8(k_cache, v_cache, k_exp, v_exp, num_blocks, block_size, num_kv_heads,
+                              head_dim);
+  if (st != NKV_OK) return st;
+  if (!block_tables || !cu_seqlens || !k_out || !v_out) return NKV_ERR_INVALID_ARGUMENT;
+  const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (k_out_stride < row || v_out_stride < row) return NKV_ERR_INVALID_ARGUMENT;
+  if ((k_out_stride % 8) != 0 || (v_out_stride % 8) != 0 || !aligned16(k_out) || !aligned16(v_out))
+    return NKV_ERR_ALIGNMENT;
+  nkv::Rows8Params p{};
+  p.cache[0] = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+  p.cache[1] = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  p.exps[0] = static_cast<uint8_t*>(const_cast<void*>(k_exp));
+  p.exps[1] = static_cast<uint8_t*>(const_cast<void*>(v_exp));
+  p.num_blocks = num_blocks;
+  p.num_kv_heads = num_kv_heads;
+  p.block_size = block_size;
+  p.dst[0] = static_cast<__nv_bfloat16*>(k_out);
+  p.dst[1] = static_cast<__nv_bfloat16*>(v_out);
+  p.dst_stride[0] = k_out_stride;
+  p.dst_stride[1] = v_out_stride;
+  p.block_tables = block_tables;
+  p.cu_seqlens = cu_seqlens;
+  p.max_blocks = max_blocks;
+  p.batch = batch;
+  p.num_rows = num_tokens * 2 * num_kv_heads;
+  return launch_rows8(nkv::load_kvcache_fp8_kernel, p, stream);
+}
+
+size_t nkv_paged_decode_fp8_workspace_size(int32_t num_q_heads, int32_t num_kv_heads) {
+  if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0) return 0;
+  return 256;
+}
+
+int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride_head,
+                         const void* k_cache, const void* v_cache, const void* k_exp,
+                         const void* v_exp, int64_t num_blocks, const int32_t* block_tables,
+                         int32_t max_blocks, const int32_t* context_lens, void* out,
+                         int64_t out_stride_token, int32_t batch, int32_t num_q_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                         float softmax_scale, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  if (batch < 0 || max_blocks < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      num_q_heads % num_kv_heads != 0)
+    return NKV_ERR_INVALID_ARGUMENT;
+  if (batch == 0) return NKV_OK;
+  const int st = check_cache8(k_cache, v_cache, k_exp, v_exp, num_blocks, block_size, num_kv_heads,
+                              head_dim);
+  if (st != NKV_OK) return st;
+  const int g = num_q_heads / num_kv_heads;
+  if (g > 16) return NKV_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(batch) * num_kv_heads > kMaxDecodePairs ||
+      static_cast<int64_t>(max_blocks) * block_size > 0x7fffffff)
+    return NKV_ERR_UNSUPPORTED;
+  if (!q || !out || !context_lens || (!block_tables && max_blocks > 0))
+    return NKV_ERR_INVALID_ARGUMENT;
+  if (!std::isfinite(softmax_scale) || !(softmax_scale > 0.f)) return NKV_ERR_INVALID_ARGUMENT;
+  if (!aligned16(q) || !aligned16(out) || (q_stride_token % 8) || (q_stride_head % 8) ||
+      (out_stride_token % 8))
+    return NKV_ERR_ALIGNMENT;
+  if (out_stride_token < static_cast<int64_t>(num_q_heads) * head_dim ||
+      q_stride_head < head_dim)
+    return NKV_ERR_INVALID_ARGUMENT;
+  const size_t need = nkv_paged_decode_fp8_workspace_size(num_q_heads, num_kv_heads);
+  if (!workspace || workspace_bytes < need) return NKV_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return NKV_ERR_ALIGNMENT;
+  nkv::Decode8Params p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride_token = q_stride_token;
+  p.q_stride_head = q_stride_head;
+  p.k_cache = static_cast<const uint8_t*>(k_cache);
+  p.v_cache = static_cast<const uint8_t*>(v_cache);
+  p.k_exp = static_cast<const uint8_t*>(k_exp);
+  p.v_exp = static_cast<const uint8_t*>(v_exp);
+  p.num_blocks = num_blocks;
+  p.block_tables = block_tables;
+  p.context_lens = context_lens;
+  p.max_blocks = max_blocks;
+  p.block_size = block_size;
+  p.batch = batch;
+  p.num_kv_heads = num_kv_heads;
+  p.g = g;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_stride_token = out_stride_token;
+  switch (padded_group(g)) {
+    case 1: return launch_decode8<1>(p, stream);
+    case 2: return launch_decode8<2>(p, stream);
+    case 4: return launch_decode8<4>(p, stream);
+    case 8: return launch_decode8<8>(p, stream);
+    default: return launch_decode8<16>(p, stream);
+  }
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- cache pages
+namespace {
+
+constexpr int kMaxPageRegions = 256;
+
+// Workspace of the page calls: [moves: PageMove x n][int32 x (n + 4)][remap: int32 x num_pages].
+struct PageWorkspace {
+  size_t off_list, off_remap, total;
+};
+PageWorkspace page_workspace(int64_t n, int64_t num_pages) {
+  PageWorkspace w;
+  w.off_list = align256(sizeof(nkv::PageMove) * static_cast<size_t>(n));
+  w.off_remap = w.off_list + align256(sizeof(int32_t) * static_cast<size_t>(n + 4));
+  w.total = w.off_remap + align256(sizeof(int32_t) * static_cast<size_t>(num_pages));
+  return w;
+}
+
+// Checks the caller's regions and lays out their copy items.
+template <int N>
+int make_regions(const nkv_page_region* in, int num, int64_t num_pages, int block_size,
+                 nkv::PageRegions<N>* out) {
+  int64_t items = 0;
+  for (int i = 0; i < num; ++i) {
+    const nkv_page_region& r = in[i];
+    if (!r.base || r.lead < 0 || r.page_bytes <= 0 || r.seg_bytes <= 0 || r.token_bytes <= 0 ||
+        r.page_bytes % r.seg_bytes != 0 || (block_size > 0 && r.seg_bytes != block_size * r.token_bytes) ||
+        (r.lead > 1 && r.lead_stride < num_pages * r.page_bytes))
+      return NKV_ERR_INVALID_ARGUMENT;
+    if (!aligned16(r.base) || r.lead_stride % 16 != 0 || r.seg_bytes % 16 != 0)
+      return NKV_ERR_ALIGNMENT;
+    nkv::PageRegion& o = out->r[i];
+    o.base = static_cast<uint8_t*>(r.base);
+    o.lead_stride = r.lead_stride;
+    o.page_bytes = r.page_bytes;
+    o.seg_bytes = r.seg_bytes;
+    o.token_bytes = r.token_bytes;
+    o.first_item = items;
+    o.items_per_page = static_cast<int>((r.page_bytes + nkv::kPageCopyBytes - 1) / nkv::kPageCopyBytes);
+    items += r.lead * o.items_per_page;
+  }
+  out->num = num;
+  out->items_per_move = items;
+  return NKV_OK;
+}
+
+template <int N>
+int launch_page_copy_n(const nkv_page_region* regions, int num, int64_t num_pages, int block_size,
+                       const nkv::PageMove* moves, const int32_t* num_moves_dev, int64_t num_moves,
+                       void* stream) {
+  nkv::PageRegions<N> rg;
+  const int st = make_regions(regions, num, num_pages, block_size, &rg);
+  if (st != NKV_OK) return st;
+  const int64_t items = rg.items_per_move * num_moves;
+  if (items == 0) return NKV_OK;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int64_t grid = std::min<int64_t>(items, static_cast<int64_t>(sm_count(dev)) * 8);
+  return launch_dependent(nkv::page_copy_kernel<N>, dim3(static_cast<unsigned>(grid)),
+                          dim3(nkv::kPageCopyThreads), 0, static_cast<cudaStream_t>(stream), rg,
+                          moves, num_moves_dev, static_cast<int>(num_moves), block_size);
+}
+
+int launch_page_copy(const nkv_page_region* regions, int num, int64_t num_pages, int block_size,
+                     const nkv::PageMove* moves, const int32_t* num_moves_dev, int64_t num_moves,
+                     void* stream) {
+  if (num == 0) return NKV_OK;
+  if (num <= 8)
+    return launch_page_copy_n<8>(regions, num, num_pages, block_size, moves, num_moves_dev,
+                                 num_moves, stream);
+  return launch_page_copy_n<kMaxPageRegions>(regions, num, num_pages, block_size, moves,
+                                             num_moves_dev, num_moves, stream);
+}
+
+// Regions are checked before anything is launched.
+int check_regions(const nkv_page_region* regions, int32_t num, int64_t num_pages, int block_size) {
+  if (num < 0 || (num > 0 && !regions)) return NKV_ERR_INVALID_ARGUMENT;
+  if (num > kMaxPageRegions || num_pages > 0x7fffffff) return NKV_ERR_UNSUPPORTED;
+  nkv::PageRegions<kMaxPageRegions> rg;
+  return make_regions(regions, num, num_pages, block_size, &rg);
+}
+
+// Dynamic shared memory for three bit maps over `count` rows or pages.
+constexpr size_t kMaxPlanSmem = 200 * 1024;
+size_t plan_smem(int64_t count) { return 3 * sizeof(uint32_t) * static_cast<size_t>((count + 31) / 32); }
+
+template <typename Params>
+int launch_plan(void (*kernel)(Params), const Params& p, size_t smem, bool* attr_set, void* stream) {
+  if (smem > 48 * 1024) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= kMaxDevices) return NKV_ERR_CUDA;
+    if (!attr_set[dev]) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(kMaxPlanSmem));
+      if (e != cudaSuccess) return cuda_status(e);
+      attr_set[dev] = true;
+    }
+  }
+  return launch_dependent(kernel, dim3(1), dim3(nkv::kPagePlanThreads), smem,
+                          static_cast<cudaStream_t>(stream), p);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t nkv_pages_workspace_size(int64_t n, int64_t num_pages) {
+  if (n < 0 || num_pages < 0 || n > 0x7fffffff || num_pages > 0x7fffffff) return 0;
+  return page_workspace(n, num_pages).total;
+}
+
+int nkv_copy_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
+                   const int32_t* src, const int32_t* dst, int32_t n, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  if (n < 0 || num_pages < 0) return NKV_ERR_INVALID_ARGUMENT;
+  const int st = check_regions(regions, num_regions, num_pages, 0);
+  if (st != NKV_OK) return st;
+  if (n == 0 || num_pages == 0) return NKV_OK;
+  if (!src || !dst) return NKV_ERR_INVALID_ARGUMENT;
+  if (plan_smem(num_pages) > kMaxPlanSmem) return NKV_ERR_UNSUPPORTED;
+  const PageWorkspace w = page_workspace(n, 0);
+  if (!workspace || workspace_bytes < w.total) return NKV_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return NKV_ERR_ALIGNMENT;
+  nkv::PageCopyPlanParams p{};
+  p.src = src;
+  p.dst = dst;
+  p.n = n;
+  p.num_pages = num_pages;
+  p.block_size = 0x7fffffff;  // every token
+  p.moves = static_cast<nkv::PageMove*>(workspace);
+  static bool attr_set[kMaxDevices] = {false};
+  const int e = launch_plan(nkv::page_copy_plan_kernel, p, plan_smem(num_pages), attr_set, stream);
+  if (e != NKV_OK) return e;
+  return launch_page_copy(regions, num_regions, num_pages, 0, p.moves, nullptr, n, stream);
+}
+
+int nkv_fork_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
+                   int32_t block_size, int32_t* block_tables, int32_t max_blocks, int32_t num_rows,
+                   int32_t* context_lens, int32_t* ref_counts, const int32_t* src_rows,
+                   const int32_t* dst_rows, int32_t n, int32_t* out_pages, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  if (n < 0 || num_pages < 0 || block_size <= 0 || max_blocks < 0 || num_rows < 0)
+    return NKV_ERR_INVALID_ARGUMENT;
+  const int st = check_regions(regions, num_regions, num_pages, block_size);
+  if (st != NKV_OK) return st;
+  if (n == 0) return NKV_OK;
+  if (!block_tables || !context_lens || !ref_counts || !src_rows || !dst_rows || !out_pages)
+    return NKV_ERR_INVALID_ARGUMENT;
+  if (plan_smem(num_rows) > kMaxPlanSmem) return NKV_ERR_UNSUPPORTED;
+  const PageWorkspace w = page_workspace(n, 0);
+  if (!workspace || workspace_bytes < w.total) return NKV_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return NKV_ERR_ALIGNMENT;
+  nkv::PageForkParams p{};
+  p.block_tables = block_tables;
+  p.max_blocks = max_blocks;
+  p.num_rows = num_rows;
+  p.context_lens = context_lens;
+  p.ref_counts = ref_counts;
+  p.num_pages = num_pages;
+  p.block_size = block_size;
+  p.src_rows = src_rows;
+  p.dst_rows = dst_rows;
+  p.n = n;
+  p.out_pages = out_pages;
+  p.moves = static_cast<nkv::PageMove*>(workspace);
+  p.free_list = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + w.off_list);
+  static bool attr_set[kMaxDevices] = {false};
+  const int e = launch_plan(nkv::page_fork_plan_kernel, p, plan_smem(num_rows), attr_set, stream);
+  if (e != NKV_OK) return e;
+  return launch_page_copy(regions, num_regions, num_pages, block_size, p.moves, nullptr, n, stream);
+}
+
+int nkv_free_pages(int32_t* block_tables, int32_t max_blocks, int32_t num_rows,
+                   int32_t* context_lens, int32_t* ref_counts, int64_t num_pages,
+                   int32_t block_size, const int32_t* rows, int32_t n, int32_t trim,
+                   void* stream) {
+  if (n < 0 || num_pages < 0 || block_size <= 0 || max_blocks < 0 || num_rows < 0)
+    return NKV_ERR_INVALID_ARGUMENT;
+  if (n == 0) return NKV_OK;
+  if (!block_tables || !context_lens || !ref_counts || !rows) return NKV_ERR_INVALID_ARGUMENT;
+  if (num_pages > 0x7fffffff) return NKV_ERR_UNSUPPORTED;
+  nkv::PageFreeParams p{};
+  p.block_tables = block_tables;
+  p.max_blocks = max_blocks;
+  p.num_rows = num_rows;
+  p.context_lens = context_lens;
+  p.ref_counts = ref_counts;
+  p.num_pages = num_pages;
+  p.block_size = block_size;
+  p.rows = rows;
+  p.n = n;
+  p.trim = trim;
+  return launch_dependent(nkv::page_free_kernel, dim3(n), dim3(256), 0,
+                          static_cast<cudaStream_t>(stream), p);
+}
+
+int nkv_compact_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
+                      const int32_t* block_tables, int32_t* out_block_tables, int64_t num_entries,
+                      const int32_t* ref_counts, int32_t* out_ref_counts, int32_t* out_num_live,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  if (num_pages < 0 || num_entries < 0) return NKV_ERR_INVALID_ARGUMENT;
+  const int st = check_regions(regions, num_regions, num_pages, 0);
+  if (st != NKV_OK) return st;
+  if (num_pages == 0) return NKV_ERR_INVALID_ARGUMENT;
+  if (!ref_counts || !out_ref_counts || !out_num_live ||
+      (num_entries > 0 && (!block_tables || !out_block_tables)))
+    return NKV_ERR_INVALID_ARGUMENT;
+  const int64_t most = num_pages / 2;  // a move needs a live page and a free one
+  const PageWorkspace w = page_workspace(most, num_pages);
+  if (!workspace || workspace_bytes < w.total) return NKV_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return NKV_ERR_ALIGNMENT;
+  nkv::PageCompactParams p{};
+  p.block_tables = block_tables;
+  p.out_block_tables = out_block_tables;
+  p.entries = num_entries;
+  p.ref_counts = ref_counts;
+  p.out_ref_counts = out_ref_counts;
+  p.num_pages = num_pages;
+  p.block_size = 0x7fffffff;
+  p.out_num_live = out_num_live;
+  p.moves = static_cast<nkv::PageMove*>(workspace);
+  p.num_moves = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + w.off_list);
+  p.remap = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + w.off_remap);
+  int e = launch_dependent(nkv::page_compact_plan_kernel, dim3(1), dim3(nkv::kPagePlanThreads), 0,
+                           static_cast<cudaStream_t>(stream), p);
+  if (e != NKV_OK) return e;
+  if (num_entries > 0) {
+    const int64_t blocks = (num_entries + 255) / 256;
+    if (blocks > 0x7fffffff) return NKV_ERR_UNSUPPORTED;
+    e = launch_dependent(nkv::page_remap_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
+                         static_cast<cudaStream_t>(stream), p);
+    if (e != NKV_OK) return e;
+  }
+  return launch_page_copy(regions, num_regions, num_pages, 0, p.moves, p.num_moves, most, stream);
+}
+
+}  // extern "C"

@@ -31,6 +31,7 @@ DEVERR_RING_RANGE = 0x10
 DEVERR_PREFILL_RANGE = 0x20
 DEVERR_ROPE_POSITION = 0x40
 DEVERR_LAUNCH_SHAPE = 0x80
+DEVERR_PAGES = 0x100
 
 # Size of the library's fixed decode scratch (NKV_STATIC_SCRATCH_BYTES, nkv.h).
 STATIC_SCRATCH_BYTES = 16 << 20
@@ -109,6 +110,40 @@ SIGNATURES: dict[str, tuple] = {
         [_P, c_int32, c_int32, c_int32, c_int32, _I32P, _P, _P, c_int64, _I32P, c_int32,
          _I32P, _I32P, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
          c_float, _I32P, _P, _P],
+    ),
+    "nkv_store_kvcache_fp8": (
+        c_int,
+        [_P, c_int64, _P, c_int64, _P, _P, _P, _P, c_int64, c_int32, _I32P, c_int32, c_int32,
+         c_int32, _P],
+    ),
+    "nkv_load_kvcache_fp8": (
+        c_int,
+        [_P, _P, _P, _P, c_int64, c_int32, _I32P, c_int32, _I32P, c_int32, c_int64, _P, c_int64,
+         _P, c_int64, c_int32, c_int32, _P],
+    ),
+    "nkv_paged_decode_fp8_workspace_size": (c_size_t, [c_int32, c_int32]),
+    "nkv_paged_decode_fp8": (
+        c_int,
+        [_P, c_int64, c_int64, _P, _P, _P, _P, c_int64, _I32P, c_int32, _I32P, _P, c_int64,
+         c_int32, c_int32, c_int32, c_int32, c_int32, c_float, _P, c_size_t, _P],
+    ),
+    "nkv_pages_workspace_size": (c_size_t, [c_int64, c_int64]),
+    "nkv_copy_pages": (
+        c_int,
+        [_P, c_int32, c_int64, _I32P, _I32P, c_int32, _P, c_size_t, _P],
+    ),
+    "nkv_fork_pages": (
+        c_int,
+        [_P, c_int32, c_int64, c_int32, _I32P, c_int32, c_int32, _I32P, _I32P, _I32P, _I32P,
+         c_int32, _I32P, _P, c_size_t, _P],
+    ),
+    "nkv_free_pages": (
+        c_int,
+        [_I32P, c_int32, c_int32, _I32P, _I32P, c_int64, c_int32, _I32P, c_int32, c_int32, _P],
+    ),
+    "nkv_compact_pages": (
+        c_int,
+        [_P, c_int32, c_int64, _I32P, _I32P, c_int64, _I32P, _I32P, _I32P, _P, c_size_t, _P],
     ),
 }
 

@@ -29,6 +29,13 @@ __all__ = [
     "window_select",
     "query_window_append",
     "threshold_compress",
+    "store_kvcache_fp8",
+    "load_kvcache_fp8",
+    "paged_decode_fp8",
+    "copy_pages",
+    "fork_pages",
+    "free_pages",
+    "compact_pages",
 ]
 
 
@@ -457,3 +464,315 @@ def threshold_compress(ring: torch.Tensor, ring_slot_of_selected: torch.Tensor, 
         block_tables.size(1), context_lens.data_ptr(), selected.data_ptr(), m, S, R, Hq, Hk, D,
         block_size, float(softmax_scale), _ptr(out_keep_idx), _ptr(out_importance),
         _stream(k_cache.device)))
+
+
+# ---------------------------------------------------------------- 8-bit cache
+def _one_device(name: str, first: torch.Tensor, *tensors: torch.Tensor | None) -> torch.device:
+    """The CUDA device all tensors are on."""
+    device = first.device
+    if device.type != "cuda":
+        raise ValueError(f"{name}: CUDA tensors required (libnkv has no CPU path)")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: all tensors must be on one CUDA device")
+    return device
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """Entry point `name` on the device's current stream, with that device current."""
+    fn = getattr(_lib.load(), name)
+    if device.index == torch.cuda.current_device():
+        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(name, status)
+
+
+def _check_cache8(k_cache, v_cache, k_exp, v_exp) -> tuple[int, int, int, int]:
+    """(num_blocks, block_size, Hk, D) of an 8-bit cache."""
+    num_blocks, block_size, Hk, D = k_cache.shape
+    assert v_cache.shape == k_cache.shape
+    assert k_cache.dtype == torch.float8_e4m3fn and v_cache.dtype == torch.float8_e4m3fn
+    assert k_exp.shape == (num_blocks, Hk, block_size) and v_exp.shape == k_exp.shape
+    assert k_exp.dtype == torch.uint8 and v_exp.dtype == torch.uint8
+    assert k_cache.is_contiguous() and v_cache.is_contiguous()
+    assert k_exp.is_contiguous() and v_exp.is_contiguous()
+    return num_blocks, block_size, Hk, D
+
+
+def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor,
+                      slot_mapping: torch.Tensor) -> None:
+    """Writes key / value rows into the slots of an 8-bit cache (slot == -1 is
+    skipped): e4m3 values with a power-of-two scale per (token, kv head) row.
+
+    key / value: [N, Hk, 128] bf16, heads contiguous, row stride free (the
+    slices of a qkv projection's output); k_cache / v_cache:
+    [num_blocks, block_size, Hk, 128] float8_e4m3fn; k_exp / v_exp:
+    [num_blocks, Hk, block_size] uint8, a row reads as
+    e4m3 * 2^(exp - 127); slot_mapping: [N] int32.
+    """
+    device = _one_device("store_kvcache_fp8", key, value, k_cache, v_cache, k_exp, v_exp,
+                         slot_mapping)
+    N, num_heads, head_dim = key.shape
+    num_blocks, block_size, Hk, D = _check_cache8(k_cache, v_cache, k_exp, v_exp)
+    assert value.shape == key.shape and (num_heads, head_dim) == (Hk, D)
+    assert key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16
+    assert key.stride(-1) == 1 and value.stride(-1) == 1
+    assert key.stride(1) == D and value.stride(1) == D
+    assert slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous()
+    assert slot_mapping.numel() == N
+    if N == 0 or num_blocks == 0:
+        return
+    _call(device, "nkv_store_kvcache_fp8", key.data_ptr(), key.stride(0), value.data_ptr(),
+          value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(),
+          v_exp.data_ptr(), num_blocks, block_size, slot_mapping.data_ptr(), N, Hk, D)
+
+
+def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor,
+                     v_exp: torch.Tensor, block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
+                     num_tokens: int, k_out: torch.Tensor | None = None,
+                     v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Whole sequences of an 8-bit cache as packed bf16 rows (exact), the k / v
+    that paged_prefill takes without a block table.
+
+    block_tables: [B, max_blocks] int32; cu_seqlens: [B + 1] int32 on the
+    device; num_tokens: rows of the outputs, at least cu_seqlens[-1] (rows
+    behind the last sequence are left as they are). Returns (k, v)
+    [num_tokens, Hk, 128] bf16.
+    """
+    device = _one_device("load_kvcache_fp8", k_cache, v_cache, k_exp, v_exp, block_tables,
+                         cu_seqlens, k_out, v_out)
+    num_blocks, block_size, Hk, D = _check_cache8(k_cache, v_cache, k_exp, v_exp)
+    B = cu_seqlens.numel() - 1
+    assert cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and B >= 0
+    assert block_tables.dtype == torch.int32 and block_tables.dim() == 2
+    assert block_tables.size(0) >= B and num_tokens >= 0
+    if not block_tables.is_contiguous():
+        block_tables = block_tables.contiguous()
+    if k_out is None:
+        k_out = torch.empty(num_tokens, Hk, D, dtype=torch.bfloat16, device=device)
+    if v_out is None:
+        v_out = torch.empty(num_tokens, Hk, D, dtype=torch.bfloat16, device=device)
+    for out in (k_out, v_out):
+        assert out.shape == (num_tokens, Hk, D) and out.dtype == torch.bfloat16
+        assert out.stride(-1) == 1 and out.stride(1) == D
+    if B == 0 or num_tokens == 0:
+        return k_out, v_out
+    _call(device, "nkv_load_kvcache_fp8", k_cache.data_ptr(), v_cache.data_ptr(),
+          k_exp.data_ptr(), v_exp.data_ptr(), num_blocks, block_size, block_tables.data_ptr(),
+          block_tables.size(1), cu_seqlens.data_ptr(), B, num_tokens, k_out.data_ptr(),
+          k_out.stride(0), v_out.data_ptr(), v_out.stride(0), Hk, D)
+    return k_out, v_out
+
+
+def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     k_exp: torch.Tensor, v_exp: torch.Tensor, block_tables: torch.Tensor,
+                     context_lens: torch.Tensor, softmax_scale: float,
+                     out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_decode over an 8-bit cache: attention of one query token per
+    sequence, split over the cached length and joined.
+
+    q: [B, Hq, 128] bf16 (row and head strides multiples of 8); the cache as
+    store_kvcache_fp8 writes it; block_tables [B, max_blocks] int32;
+    context_lens [B] int32 (0 gives zeros). workspace (uint8, at least
+    decode_fp8_workspace_bytes) may hold anything; by default every call takes
+    its own from torch's allocator, so calls on several streams and captured
+    graphs share none. Returns out [B, Hq, 128] bf16.
+    """
+    device = _one_device("paged_decode_fp8", q, k_cache, v_cache, k_exp, v_exp, block_tables,
+                         context_lens, out, workspace)
+    B, Hq, D = q.shape
+    num_blocks, block_size, Hk, Dk = _check_cache8(k_cache, v_cache, k_exp, v_exp)
+    assert Dk == D and Hk > 0 and Hq % Hk == 0
+    assert q.dtype == torch.bfloat16 and q.stride(-1) == 1
+    assert block_tables.dtype == torch.int32 and context_lens.dtype == torch.int32
+    assert block_tables.dim() == 2 and block_tables.size(0) >= B
+    assert context_lens.numel() >= B and context_lens.is_contiguous()
+    if not block_tables.is_contiguous():
+        block_tables = block_tables.contiguous()
+    if out is None:
+        out = torch.empty(B, Hq, D, dtype=torch.bfloat16, device=device)
+    assert out.shape == q.shape and out.dtype == torch.bfloat16
+    assert out.stride(-1) == 1 and out.stride(1) == D
+    if B == 0:
+        return out
+    if workspace is None:
+        workspace = torch.empty(decode_fp8_workspace_bytes(Hq, Hk), dtype=torch.uint8,
+                                device=device)
+    assert workspace.is_contiguous()
+    _call(device, "nkv_paged_decode_fp8", q.data_ptr(), q.stride(0), q.stride(1),
+          k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), num_blocks,
+          block_tables.data_ptr(), block_tables.size(1), context_lens.data_ptr(), out.data_ptr(),
+          out.stride(0), B, Hq, Hk, D, block_size, float(softmax_scale), workspace.data_ptr(),
+          workspace.numel() * workspace.element_size())
+    return out
+
+
+def decode_fp8_workspace_bytes(num_q_heads: int, num_kv_heads: int) -> int:
+    return int(_lib.load().nkv_paged_decode_fp8_workspace_size(num_q_heads, num_kv_heads))
+
+
+# ---------------------------------------------------------------- pages
+_MAX_PAGE_REGIONS = 256
+
+
+def _page_regions(caches, page_dim: int, num_pages: int | None,
+                  block_size: int | None) -> tuple[torch.Tensor | None, int, int | None]:
+    """The caches as nkv_page_region records: (host int64 [n, 6], n, num_pages).
+
+    Each cache is contiguous, [*lead, num_pages, *page] with page_dim leading
+    dims; with a block size a page is [block_size, Hk, D] (values) or
+    [Hk, block_size] (exponent bytes)."""
+    rows = []
+    for c in caches:
+        assert c.is_contiguous() and 0 <= page_dim < c.dim()
+        if num_pages is None:
+            num_pages = c.size(page_dim)
+        assert c.size(page_dim) == num_pages, "the caches differ in their number of pages"
+        size = c.element_size()
+        lead = math.prod(c.shape[:page_dim])
+        page = c.shape[page_dim + 1:]
+        page_bytes = math.prod(page) * size
+        if block_size is None:
+            seg_bytes = token_bytes = page_bytes
+        elif len(page) == 3:
+            assert page[0] == block_size
+            token_bytes = page[1] * page[2] * size
+            seg_bytes = page_bytes
+        else:
+            assert len(page) == 2 and page[1] == block_size
+            token_bytes = size
+            seg_bytes = block_size * size
+        rows.append((c.data_ptr(), lead, num_pages * page_bytes, page_bytes, seg_bytes,
+                     token_bytes))
+    if not rows:
+        return None, 0, num_pages
+    return torch.tensor(rows, dtype=torch.int64), len(rows), num_pages
+
+
+def _check_page_state(block_tables, context_lens, ref_counts) -> None:
+    for t in (block_tables, context_lens, ref_counts):
+        assert t is None or (t.dtype == torch.int32 and t.is_contiguous())
+    assert block_tables.dim() == 2
+    assert context_lens is None or context_lens.numel() == block_tables.size(0)
+
+
+def _check_index(*tensors: torch.Tensor) -> int:
+    n = tensors[0].numel()
+    for t in tensors:
+        assert t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n
+    return n
+
+
+def _pages_workspace(device: torch.device, n: int, num_pages: int) -> torch.Tensor:
+    """Scratch of one page call, from torch's allocator (stream-ordered, and a
+    captured graph's own)."""
+    return torch.empty(int(_lib.load().nkv_pages_workspace_size(n, num_pages)), dtype=torch.uint8,
+                       device=device)
+
+
+def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor, page_dim: int = 0) -> None:
+    """Copies page src[i] to page dst[i] in every cache tensor.
+
+    caches: contiguous CUDA tensors [*lead, num_pages, *page] with page_dim
+    leading dims (0 for one layer's view, 2 for kv_cache[2, layers, ...]);
+    src / dst: int32 on the device. A page may be a source many times; a pair
+    whose target is another pair's target or source, or outside the cache, is
+    not copied and sets DEVERR_PAGES. Pairs (-1, -1) are padding.
+    """
+    caches = list(caches)
+    device = _one_device("copy_pages", src, dst, *caches)
+    n = _check_index(src, dst)
+    regions, count, num_pages = _page_regions(caches, page_dim, None, None)
+    if n == 0 or count == 0:
+        return
+    ws = _pages_workspace(device, n, 0)
+    _call(device, "nkv_copy_pages", regions.data_ptr(), count, num_pages, src.data_ptr(),
+          dst.data_ptr(), n, ws.data_ptr(), ws.numel())
+
+
+def fork_pages(caches, block_tables: torch.Tensor, context_lens: torch.Tensor,
+               ref_counts: torch.Tensor, src_rows: torch.Tensor, dst_rows: torch.Tensor,
+               block_size: int, page_dim: int = 0,
+               out_pages: torch.Tensor | None = None) -> torch.Tensor:
+    """Row dst_rows[i] becomes a copy of row src_rows[i]: full pages shared
+    (ref_counts + 1), a partial last page copied -- its tokens only -- to the
+    lowest free page (ref_counts <= 0); the pages dst_rows held are released
+    first.
+
+    block_tables [rows, max_blocks], context_lens [rows] and ref_counts
+    [num_pages] (all int32) are updated in place; caches as copy_pages, each
+    page [block_size, Hk, D] or, for exponent bytes, [Hk, block_size].
+    Returns out_pages int32 [n]: the page that was taken, -1 if none was
+    needed, -2 if the fork was not made (a target that is named twice or is a
+    source, a row out of range, no free page: DEVERR_PAGES is set; or a
+    (-1, -1) padding pair).
+    """
+    caches = list(caches)
+    device = _one_device("fork_pages", block_tables, context_lens, ref_counts, src_rows, dst_rows,
+                         out_pages, *caches)
+    _check_page_state(block_tables, context_lens, ref_counts)
+    n = _check_index(src_rows, dst_rows)
+    num_pages = ref_counts.numel()
+    regions, count, _ = _page_regions(caches, page_dim, num_pages, block_size)
+    if out_pages is None:
+        out_pages = torch.empty(n, dtype=torch.int32, device=device)
+    assert out_pages.dtype == torch.int32 and out_pages.is_contiguous() and out_pages.numel() == n
+    if n == 0:
+        return out_pages
+    ws = _pages_workspace(device, n, 0)
+    _call(device, "nkv_fork_pages", _ptr(regions), count, num_pages, block_size,
+          block_tables.data_ptr(), block_tables.size(1), block_tables.size(0),
+          context_lens.data_ptr(), ref_counts.data_ptr(), src_rows.data_ptr(),
+          dst_rows.data_ptr(), n, out_pages.data_ptr(), ws.data_ptr(), ws.numel())
+    return out_pages
+
+
+def free_pages(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_counts: torch.Tensor,
+               rows: torch.Tensor, block_size: int, trim: bool = False) -> None:
+    """The named rows (int32 on the device, -1 is padding) give up their pages:
+    ref_counts - 1, table entries -1. trim=False: all pages, and the row's
+    length becomes 0; trim=True: the pages past context_lens, as after a
+    compression that shortened the rows on the device."""
+    device = _one_device("free_pages", block_tables, context_lens, ref_counts, rows)
+    _check_page_state(block_tables, context_lens, ref_counts)
+    n = _check_index(rows)
+    if n == 0:
+        return
+    _call(device, "nkv_free_pages", block_tables.data_ptr(), block_tables.size(1),
+          block_tables.size(0), context_lens.data_ptr(), ref_counts.data_ptr(),
+          ref_counts.numel(), block_size, rows.data_ptr(), n, 1 if trim else 0)
+
+
+def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, page_dim: int = 0,
+                  out_block_tables: torch.Tensor | None = None,
+                  out_ref_counts: torch.Tensor | None = None,
+                  out_num_live: torch.Tensor | None = None) -> torch.Tensor:
+    """Brings the n pages in use (ref_counts > 0) to the first n of the cache:
+    the i-th used page at or past n moves to the i-th free page before n in
+    every cache tensor, and tables and counts follow (in place, or into the
+    out tensors). Returns out_num_live, int32 [1]: n."""
+    caches = list(caches)
+    device = _one_device("compact_pages", block_tables, ref_counts, out_block_tables,
+                         out_ref_counts, out_num_live, *caches)
+    if out_block_tables is None:
+        out_block_tables = block_tables
+    if out_ref_counts is None:
+        out_ref_counts = ref_counts
+    _check_page_state(block_tables, None, ref_counts)
+    _check_page_state(out_block_tables, None, out_ref_counts)
+    assert out_block_tables.shape == block_tables.shape
+    assert out_ref_counts.numel() == ref_counts.numel()
+    if out_num_live is None:
+        out_num_live = torch.empty(1, dtype=torch.int32, device=device)
+    assert out_num_live.dtype == torch.int32 and out_num_live.numel() == 1
+    num_pages = ref_counts.numel()
+    regions, count, _ = _page_regions(caches, page_dim, num_pages, None)
+    ws = _pages_workspace(device, num_pages // 2, num_pages)
+    _call(device, "nkv_compact_pages", _ptr(regions), count, num_pages, block_tables.data_ptr(),
+          out_block_tables.data_ptr(), block_tables.numel(), ref_counts.data_ptr(),
+          out_ref_counts.data_ptr(), out_num_live.data_ptr(), ws.data_ptr(), ws.numel())
+    return out_num_live
