@@ -1312,10 +1312,47 @@ int launch_rows8(void (*kernel)(nkv::Rows8Params), const nkv::Rows8Params& p, vo
                           0, static_cast<cudaStream_t>(stream), p);
 }
 
+// 8-bit map of a cache {128 values, kv heads, slots}, boxes of `rows` slots of
+// one head, 128-byte swizzle.
+int encode_cache8(CUtensorMap* map, const void* base, int num_kv_heads, int64_t slots, int rows) {
+  auto fn = encode_fn();
+  if (!fn) return NKV_ERR_CUDA;
+  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(num_kv_heads),
+                              static_cast<cuuint64_t>(slots)};
+  const cuuint64_t strides[2] = {128, static_cast<cuuint64_t>(num_kv_heads) * 128};
+  const cuuint32_t box[3] = {128, 1, static_cast<cuuint32_t>(rows)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NKV_OK : NKV_ERR_ALIGNMENT;
+}
+
+// Workspace: [split records][partials], kDecode8MaxCtas CTAs.
+constexpr size_t kDecode8SplitBytes =
+    (sizeof(nkv::Decode8Split) * nkv::kDecode8MaxCtas + 255) / 256 * 256;
+size_t decode8_workspace(int g) {
+  return kDecode8SplitBytes +
+         align256(sizeof(float) * nkv::kDecode8ORow * 2 * g * nkv::kDecode8MaxCtas);
+}
+
 template <int G>
-int launch_decode8(const nkv::Decode8Params& p, void* stream) {
-  return launch_dependent(nkv::paged_decode_fp8_kernel<G>, dim3(p.batch * p.num_kv_heads),
-                          dim3(nkv::kDecode8Warps * 32), 0, static_cast<cudaStream_t>(stream), p);
+int launch_decode8(const CUtensorMap& tk, const CUtensorMap& tv, const nkv::Decode8Params& p,
+                   int grid, cudaStream_t stream) {
+  using S = nkv::Decode8Shape<G>;
+  static_assert(S::kSmemBytes <= kSmemOptinBytes, "shared memory of the 8-bit decode");
+  static bool attr_set[kMaxDevices] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices) return NKV_ERR_CUDA;
+  if (!attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(nkv::paged_decode_fp8_kernel<G>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
+    if (e != cudaSuccess) return cuda_status(e);
+    attr_set[dev] = true;
+  }
+  return launch_dependent(nkv::paged_decode_fp8_kernel<G>, dim3(grid), dim3(nkv::kDecode8Threads),
+                          S::kSmemBytes, stream, tk, tv, p);
 }
 
 }  // namespace
@@ -1392,7 +1429,7 @@ int nkv_load_kvcache_fp8(const void* k_cache, const void* v_cache, const void* k
 
 size_t nkv_paged_decode_fp8_workspace_size(int32_t num_q_heads, int32_t num_kv_heads) {
   if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0) return 0;
-  return 256;
+  return decode8_workspace(num_q_heads / num_kv_heads);
 }
 
 int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride_head,
@@ -1431,8 +1468,6 @@ int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_stride_token = q_stride_token;
   p.q_stride_head = q_stride_head;
-  p.k_cache = static_cast<const uint8_t*>(k_cache);
-  p.v_cache = static_cast<const uint8_t*>(v_cache);
   p.k_exp = static_cast<const uint8_t*>(k_exp);
   p.v_exp = static_cast<const uint8_t*>(v_exp);
   p.num_blocks = num_blocks;
@@ -1446,13 +1481,33 @@ int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.out_stride_token = out_stride_token;
+  p.box_rows = std::min(block_size, nkv::kDecode8Tile);
+  p.splits = static_cast<nkv::Decode8Split*>(workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kDecode8SplitBytes);
+  CUtensorMap tk, tv;
+  const int64_t slots = std::max<int64_t>(num_blocks, 1) * block_size;
+  int e = encode_cache8(&tk, k_cache, num_kv_heads, slots, p.box_rows);
+  if (e == NKV_OK) e = encode_cache8(&tv, v_cache, num_kv_heads, slots, p.box_rows);
+  if (e != NKV_OK) return e;
+  // one CTA per SM, no more than there can be tiles
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int64_t row_tiles = (static_cast<int64_t>(max_blocks) * block_size + nkv::kDecode8Tile - 1) /
+                            nkv::kDecode8Tile;
+  const int64_t tiles = std::max<int64_t>(1, row_tiles * batch * num_kv_heads);
+  const int grid = static_cast<int>(std::min<int64_t>(
+      {static_cast<int64_t>(sm_count(dev)), static_cast<int64_t>(nkv::kDecode8MaxCtas), tiles}));
+  const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   switch (padded_group(g)) {
-    case 1: return launch_decode8<1>(p, stream);
-    case 2: return launch_decode8<2>(p, stream);
-    case 4: return launch_decode8<4>(p, stream);
-    case 8: return launch_decode8<8>(p, stream);
-    default: return launch_decode8<16>(p, stream);
+    case 1: e = launch_decode8<1>(tk, tv, p, grid, cs); break;
+    case 2: e = launch_decode8<2>(tk, tv, p, grid, cs); break;
+    case 4: e = launch_decode8<4>(tk, tv, p, grid, cs); break;
+    case 8: e = launch_decode8<8>(tk, tv, p, grid, cs); break;
+    default: e = launch_decode8<16>(tk, tv, p, grid, cs); break;
   }
+  if (e != NKV_OK || row_tiles <= 1 || grid == 1) return e;  // no pair can be split
+  return launch_dependent(nkv::decode_fp8_join_kernel, dim3(grid, g),
+                          dim3(nkv::kDecode8JoinWarps * 32), 0, cs, p);
 }
 
 }  // extern "C"

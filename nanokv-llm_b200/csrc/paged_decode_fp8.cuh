@@ -5,21 +5,81 @@
 // g = Hq / Hk query heads of a group share a kv head. A row of length 0 gives
 // zeros.
 //
-// One CTA per (row, kv head): four warps take the tokens in turn, a lane holds
-// four dims of each of the group's heads, with a running maximum and sum per
-// warp, merged at the end.
+// What bounds it: HBM. A cached token of a kv head is 258 bytes and 4 g * 128
+// FLOP, 2 g FLOP a byte.
+//
+// Split and join. The work of a call is the 128-token tiles of every (row, kv
+// head) pair in the order (row, head, tile); CTA c of n takes the tiles
+// [c T / n, (c + 1) T / n). Every CTA has the same number of tiles, whatever
+// the lengths, and which tiles depends on the lengths alone: results are the
+// same every time. A CTA finishes the pairs that lie inside its range; of a
+// pair that it shares with others it leaves the raw (m, l, O) in the workspace
+// (at most two: at its range's start and end), which a second kernel, launched
+// behind the first with programmatic dependence, joins in the CTAs' order. No
+// counters, so the workspace needs no content and outlives nothing.
+//
+// One CTA per SM: a producer warp walks the range and keeps a ring of tiles
+// full (TMA for K and V, 128-byte rows, 128B swizzle; bulk copies for the
+// exponent bytes and the group's q rows), four consumer warps take 32 tokens
+// of every tile each, with a running softmax per warp that is merged in shared
+// memory at the end of a pair.
+//
+// Arithmetic. e4m3 is exact in f16, so K and V go to the tensor cores as f16
+// (mma.sync m16n8k16, 32-bit accumulators; groups of 1 to 16 heads are too
+// narrow for 64-row tcgen05 tiles). Products are transposed, S^T = K Q^T and
+// O^T = V^T P^T: tokens and dims fill the 16 rows, the heads the 8 columns.
+//   * q is scaled by the power of two that brings its row's maximum into
+//     [1, 2) and rounded to f16: 11 bits for a bf16's 8, so only elements
+//     below 2^-14 of the maximum lose any (at most 2^-25 of the maximum).
+//   * K's exponents and that power of two multiply the 32-bit scores.
+//   * V's exponents go into the weights: w_j = 2^(s_j + k_j - M) with M the
+//     running maximum of s_j + k_j (s in log2 units), so w <= 1 and what matters
+//     most has f16's full 11 bits, however far the rows' scales are apart. The
+//     softmax's own maximum m and sum l are kept beside it in 32 bits; at the
+//     end O is multiplied by 2^(M - m).
+// Rows of 8-bit values come out of ldmatrix as 16-bit pairs: for K two dims of
+// a token (the k order of the product is permuted to match, in q's fragments
+// too), for V, transposed, two dims of two tokens; one byte permute makes them
+// two tokens of each dim, and the dims of a fragment's upper and lower 8 rows
+// are the odd and the even ones.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "fp8_cache.cuh"
+#include "tcgen05.cuh"
 
 namespace nkv {
 
-constexpr int kDecode8Warps = 4;
+constexpr int kDecode8Tile = 128;
+constexpr int kDecode8Warps = 4;  // consumers
+constexpr int kDecode8Threads = (kDecode8Warps + 1) * 32;
+constexpr int kDecode8TileBytes = kDecode8Tile * 128;
+constexpr int kDecode8MaxCtas = 160;
+constexpr int kDecode8ORow = 132;   // floats of one row of a partial: O[128], m, l, 2 of padding
+constexpr int kDecode8JoinWarps = 8;
+
+template <int G>
+struct Decode8Shape {
+  static_assert(G == 1 || G == 2 || G == 4 || G == 8 || G == 16, "padded group width");
+  static constexpr int kNT = G <= 8 ? 1 : 2;  // 8-head column tiles
+  static constexpr int kStages = G <= 8 ? 5 : 4;
+  static constexpr int kQBytes = (G < 4 ? 4 : G) * 256;
+  // [K][V][q rows][K exponents][V exponents], 1024-byte aligned
+  static constexpr int kStageBytes = 2 * kDecode8TileBytes + kQBytes + 1024;
+  static constexpr int kStateFloats = kDecode8Warps * G * kDecode8ORow;
+  static constexpr int kBarOffset = kStages * kStageBytes + 2 * kStateFloats * 4;
+  static constexpr int kSmemBytes = kBarOffset + (2 * kStages + 2) * 8 + kStages * 16 + 16 + 1024;
+};
+
+// What CTA c leaves for the join: the pair that begins in its range and goes
+// on in the next CTAs', and how many CTAs share it (0: none).
+struct Decode8Split {
+  int32_t pair, pieces;
+};
 
 struct Decode8Params {
   const __nv_bfloat16* q;
   int64_t q_stride_token, q_stride_head;
-  const uint8_t* k_cache;
-  const uint8_t* v_cache;
   const uint8_t* k_exp;
   const uint8_t* v_exp;
   int64_t num_blocks;
@@ -27,101 +87,573 @@ struct Decode8Params {
   const int32_t* context_lens;
   int max_blocks;
   int block_size;
+  int box_rows;   // tokens of one TMA box: min(block_size, 128)
   int batch;
   int num_kv_heads;
   int g;
   float scale_log2;
   __nv_bfloat16* out;
   int64_t out_stride_token;
+  Decode8Split* splits;  // [CTAs]
+  float* parts;          // [CTAs][2][g][kDecode8ORow]: range's first pair, last pair
 };
 
-__device__ __forceinline__ float4 e4m3x4_to_float4(uint32_t w, float s) {
-  const uint32_t a = e4m3x2_to_f16x2(w), b = e4m3x2_hi_to_f16x2(w);
-  const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a));
-  const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
-  return make_float4(fa.x * s, fa.y * s, fb.x * s, fb.y * s);
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Length of row b, kept inside its block table.
+__device__ __forceinline__ int decode8_length(const Decode8Params& p, int b) {
+  int len = max(__ldg(p.context_lens + b), 0);
+  if (len > p.max_blocks * p.block_size) {
+    raise_error(NKV_DEVERR_DECODE_BLOCK);
+    len = p.max_blocks * p.block_size;
+  }
+  return len;
+}
+
+__device__ __forceinline__ int decode8_tiles(int len) {
+  return (len + kDecode8Tile - 1) / kDecode8Tile;
+}
+
+__device__ __forceinline__ void decode8_store(__nv_bfloat16* dst, float4 v, float f) {
+  uint2 u;
+  u.x = pack_bf16x2(v.x * f, v.y * f);
+  u.y = pack_bf16x2(v.z * f, v.w * f);
+  *reinterpret_cast<uint2*>(dst) = u;
 }
 
 template <int G>
-__global__ void __launch_bounds__(kDecode8Warps * 32) paged_decode_fp8_kernel(const Decode8Params p) {
-  __shared__ float so[kDecode8Warps][G][128], sm[kDecode8Warps][G], sl[kDecode8Warps][G];
-  grid_dependency_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.x / p.num_kv_heads, h = blockIdx.x % p.num_kv_heads;
-  int len = p.context_lens[b];
-  if (len > p.max_blocks * p.block_size) {
-    if (threadIdx.x == 0) raise_error(NKV_DEVERR_DECODE_BLOCK);
-    len = p.max_blocks * p.block_size;
+__global__ void __launch_bounds__(kDecode8Threads, 1)
+paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, const Decode8Params p) {
+  using S = Decode8Shape<G>;
+  constexpr int kStages = S::kStages;
+  constexpr int kNT = S::kNT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  float* state = reinterpret_cast<float*>(smem + kStages * S::kStageBytes);  // two buffers
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kBarOffset);
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* merge_bar = empty_bar + kStages;  // one per state buffer
+  // per stage: row (-1: no more tiles), head, flags | valid tokens << 8
+  int* meta = reinterpret_cast<int*>(merge_bar + 2);
+  volatile int* abort_flag = meta + kStages * 4;
+  enum { kFirst = 1, kLast = 2, kPartial = 4, kPartialSlot1 = 8 };
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), kDecode8Warps);
+    }
+    mbar_init(smem_u32(&merge_bar[0]), kDecode8Warps);
+    mbar_init(smem_u32(&merge_bar[1]), kDecode8Warps);
+    *abort_flag = 0;
+    fence_barrier_init();
   }
-  float4 q[G], o[G];
-  float m[G], l[G];
-#pragma unroll
-  for (int r = 0; r < G; ++r) {
-    q[r] = o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-    if (r < p.g) {
-      const uint2 u = *reinterpret_cast<const uint2*>(p.q + b * p.q_stride_token +
-                                                      (h * p.g + r) * p.q_stride_head + 4 * lane);
-      q[r] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
-                         __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
-    }
-  }
-  for (int t = warp; t < len; t += kDecode8Warps) {
-    const int bi = t / p.block_size, off = t - bi * p.block_size;
-    const int32_t blk = p.block_tables[static_cast<int64_t>(b) * p.max_blocks + bi];
-    if (blk < 0 || blk >= p.num_blocks) {
-      if (lane == 0) raise_error(NKV_DEVERR_DECODE_BLOCK);
-      continue;
-    }
-    const int64_t row = ((static_cast<int64_t>(blk) * p.block_size + off) * p.num_kv_heads + h) * 128 + 4 * lane;
-    const int64_t e = (static_cast<int64_t>(blk) * p.num_kv_heads + h) * p.block_size + off;
-    const float4 k = e4m3x4_to_float4(*reinterpret_cast<const uint32_t*>(p.k_cache + row),
-                                      exp_byte_to_float(p.k_exp[e]));
-    const float4 v = e4m3x4_to_float4(*reinterpret_cast<const uint32_t*>(p.v_cache + row),
-                                      exp_byte_to_float(p.v_exp[e]));
-#pragma unroll
-    for (int r = 0; r < G; ++r) {
-      float s = q[r].x * k.x + q[r].y * k.y + q[r].z * k.z + q[r].w * k.w;
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= p.scale_log2;
-      const float m_new = fmaxf(m[r], s);
-      const float a = exp2f(m[r] - m_new), w = exp2f(s - m_new);
-      m[r] = m_new;
-      l[r] = l[r] * a + w;
-      o[r] = make_float4(o[r].x * a + w * v.x, o[r].y * a + w * v.y, o[r].z * a + w * v.z,
-                         o[r].w * a + w * v.w);
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < G; ++r) {
-    *reinterpret_cast<float4*>(&so[warp][r][4 * lane]) = o[r];
-    if (lane == 0) {
-      sm[warp][r] = m[r];
-      sl[warp][r] = l[r];
-    }
+  // exponent bytes that no copy fills (a table entry that is no page) are finite
+  for (int s = 0; s < kStages; ++s)
+    if (threadIdx.x < 16)
+      reinterpret_cast<uint4*>(smem + s * S::kStageBytes + 2 * kDecode8TileBytes + S::kQBytes)[threadIdx.x] =
+          make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async_shared();
+  if (threadIdx.x == kDecode8Warps * 32) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
   }
   __syncthreads();
-  for (int r = warp; r < p.g; r += kDecode8Warps) {
-    float M = -INFINITY, L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < kDecode8Warps; ++w) M = fmaxf(M, sm[w][r]);
-    for (int w = 0; w < kDecode8Warps; ++w) {
-      const float f = sm[w][r] == -INFINITY ? 0.f : exp2f(sm[w][r] - M);
-      const float4 x = *reinterpret_cast<const float4*>(&so[w][r][4 * lane]);
-      L += sl[w][r] * f;
-      acc.x += x.x * f;
-      acc.y += x.y * f;
-      acc.z += x.z * f;
-      acc.w += x.w * f;
+  grid_dependency_wait();
+  allow_dependent_launch();
+
+  const int Hk = p.num_kv_heads;
+  const int g = p.g;
+
+  if (warp == kDecode8Warps) {
+    // ------------------------------------------------------------ producer
+    const uint64_t policy = l2_policy_evict_first();
+    const uint32_t q_bytes = static_cast<uint32_t>(g) * 256u;
+    // ---- this CTA's range of tiles
+    int64_t total = 0;
+    for (int b = lane; b < p.batch; b += 32) total += decode8_tiles(decode8_length(p, b));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total *= Hk;
+    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
+    int64_t u = 0, left = 0;
+    if (static_cast<int64_t>(blockIdx.x) < ctas) {
+      u = blockIdx.x * total / ctas;
+      left = (blockIdx.x + 1) * total / ctas - u;
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    uint2 u;
-    u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-    u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(p.out + b * p.out_stride_token + (h * p.g + r) * 128 + 4 * lane) = u;
+    // ---- its first row, head and tile
+    int b = 0, h = 0, t = 0, len = 0, ntiles = 0;
+    if (left > 0) {
+      int64_t base = 0;
+      for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int my_len = b0 + lane < p.batch ? decode8_length(p, b0 + lane) : 0;
+        const int my_tiles = decode8_tiles(my_len);
+        int64_t incl = my_tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, (base + incl) * Hk > u);
+        if (past != 0u) {
+          const int at = __ffs(past) - 1;
+          b = b0 + at;
+          len = __shfl_sync(0xffffffffu, my_len, at);
+          ntiles = __shfl_sync(0xffffffffu, my_tiles, at);
+          const int64_t rest = u - (base + __shfl_sync(0xffffffffu, incl, at) - ntiles) * Hk;
+          h = static_cast<int>(rest / ntiles);
+          t = static_cast<int>(rest - static_cast<int64_t>(h) * ntiles);
+          break;
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    // 32 entries of the row's block table from entry win0, one per lane
+    int win0 = 0, ent = -1;
+    auto load_window = [&](int first) {
+      win0 = first;
+      ent = -1;
+      if (first + lane < p.max_blocks)
+        ent = __ldg(p.block_tables + static_cast<int64_t>(b) * p.max_blocks + first + lane);
+    };
+    if (left > 0) load_window(t * kDecode8Tile / p.block_size);
+    int stage = 0;
+    uint32_t phase = 0;
+    int64_t issued = 0;
+    bool ok = true;
+    Decode8Split split{0, 0};
+    while (left > 0 && ok) {
+      // ---- tiles [t, t + count) of (b, h)
+      const int count = static_cast<int>(min(left, static_cast<int64_t>(ntiles - t)));
+      const bool whole = count == ntiles;
+      const bool begins = t == 0;
+      if (begins && !whole) {
+        const int64_t last_tile = u + ntiles - 1;
+        split.pair = b * Hk + h;
+        split.pieces = static_cast<int>(((last_tile + 1) * ctas - 1) / total - blockIdx.x) + 1;
+      }
+      for (int j = 0; j < count; ++j) {
+        const int tok = (t + j) * kDecode8Tile;
+        const int valid = min(kDecode8Tile, len - tok);
+        const int page = tok / p.block_size;
+        const int off = tok - page * p.block_size;  // 0 when pages are shorter than a tile
+        const int pages = p.box_rows == kDecode8Tile ? 1 : (valid + p.box_rows - 1) / p.box_rows;
+        if (page + pages - 1 - win0 >= 32) load_window(page);
+        const int blk = __shfl_sync(0xffffffffu, ent, (page - win0 + lane) & 31);
+        const bool mine = lane < pages;
+        const bool good = blk >= 0 && blk < p.num_blocks;
+        const unsigned good_pages = __ballot_sync(0xffffffffu, mine && good);
+        if (mine && !good) raise_error(NKV_DEVERR_DECODE_BLOCK);
+        if (lane == 0) ok = *abort_flag == 0 && mbar_wait_bounded(smem_u32(&empty_bar[stage]), phase ^ 1u);
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) break;
+        uint8_t* sp = smem + stage * S::kStageBytes;
+        const uint32_t sbase = smem_u32(sp);
+        const uint32_t bar = smem_u32(&full_bar[stage]);
+        if (lane == 0) {
+          int* m = meta + stage * 4;
+          m[0] = b;
+          m[1] = h;
+          m[2] = (j == 0 ? kFirst : 0) | (j == count - 1 ? kLast : 0) | (whole ? 0 : kPartial) |
+                 (begins ? kPartialSlot1 : 0) | (valid << 8);
+          mbar_arrive_expect_tx(bar, static_cast<uint32_t>(pages * p.box_rows * 256) +
+                                         __popc(good_pages) * p.box_rows * 2 +
+                                         (j == 0 ? q_bytes : 0u));
+        }
+        __syncwarp();
+        if (mine) {
+          // a page that is none: rows far outside the tensor, which TMA fills with zeros
+          const int row = good ? blk * p.block_size + off : -2 * kDecode8Tile;
+          const uint32_t at = static_cast<uint32_t>(lane * p.box_rows);
+          tma_load_3d(sbase + at * 128u, &tm_k, bar, 0, h, row, policy);
+          tma_load_3d(sbase + kDecode8TileBytes + at * 128u, &tm_v, bar, 0, h, row, policy);
+          if (good) {
+            const int64_t e = (static_cast<int64_t>(blk) * Hk + h) * p.block_size + off;
+            const uint32_t se = sbase + 2 * kDecode8TileBytes + S::kQBytes + at;
+            bulk_load_row(se, p.k_exp + e, p.box_rows, bar);
+            bulk_load_row(se + kDecode8Tile, p.v_exp + e, p.box_rows, bar);
+          }
+        }
+        if (j == 0) {
+          const __nv_bfloat16* src = p.q + b * p.q_stride_token + static_cast<int64_t>(h) * g * p.q_stride_head;
+          const uint32_t sq = sbase + 2 * kDecode8TileBytes;
+          if (p.q_stride_head == 128) {
+            if (lane == 0) bulk_load_row(sq, src, q_bytes, bar);
+          } else if (lane < g) {
+            bulk_load_row(sq + lane * 256, src + lane * p.q_stride_head, 256, bar);
+          }
+        }
+        ++issued;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      u += count;
+      left -= count;
+      t = 0;
+      if (++h == Hk) {
+        h = 0;
+        // the next row that has tokens
+        while (left > 0) {
+          const int my = b + 1 + lane;
+          const int my_len = my < p.batch ? decode8_length(p, my) : 0;
+          const unsigned some = __ballot_sync(0xffffffffu, my_len > 0);
+          const int at = some != 0u ? __ffs(some) - 1 : 31;
+          b += 1 + at;
+          if (some != 0u) {
+            len = __shfl_sync(0xffffffffu, my_len, at);
+            ntiles = decode8_tiles(len);
+            break;
+          }
+        }
+        if (left > 0) load_window(0);
+      } else if (left > 0 && win0 != 0) {
+        load_window(0);
+      }
+    }
+    if (lane == 0) {
+      p.splits[blockIdx.x] = split;
+      if (ok && mbar_wait_bounded(smem_u32(&empty_bar[stage]), phase ^ 1u)) {
+        meta[stage * 4] = -1;
+        mbar_arrive(smem_u32(&full_bar[stage]));
+      } else {
+        *abort_flag = 1;
+        // after a wait that gave up: leave no copy in flight behind
+        for (int64_t i = max(issued - kStages, static_cast<int64_t>(0)); i < issued; ++i)
+          mbar_wait_bounded(smem_u32(&full_bar[i % kStages]), static_cast<uint32_t>(i / kStages) & 1u);
+      }
+    }
+    return;
   }
+
+  // -------------------------------------------------------------- consumers
+  const int gid = lane >> 2;
+  const int tig = lane & 3;
+  const float NEG_INF = -INFINITY;
+  // rows without a token
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (__ldg(p.context_lens + b) > 0 && p.max_blocks > 0) continue;
+    uint4* dst = reinterpret_cast<uint4*>(p.out + b * p.out_stride_token);
+    for (int i = threadIdx.x; i < Hk * g * 16; i += kDecode8Warps * 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+
+  float o[8][kNT][4];  // O^T: dims 16 dm + 2 gid (+ 1 for [2], [3]), heads 8 nt + 2 tig (+ 1 for odd)
+  float m_run[kNT][2], l_run[kNT][2], w_run[kNT][2];
+  uint32_t qb[8][kNT][2];
+  float qs[kNT][2];
+  int stage = 0;
+  uint32_t phase = 0;
+  uint32_t merges = 0;
+  while (true) {
+    if (!mbar_wait_bounded(smem_u32(&full_bar[stage]), phase)) {
+      *abort_flag = 1;
+      break;
+    }
+    const int b = meta[stage * 4];
+    if (b < 0) break;
+    const int h = meta[stage * 4 + 1];
+    const int flags = meta[stage * 4 + 2];
+    const int valid = flags >> 8;
+    const uint8_t* sp = smem + stage * S::kStageBytes;
+    const uint8_t* sexp = sp + 2 * kDecode8TileBytes + S::kQBytes;
+
+    if (flags & kFirst) {
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+        for (int dm = 0; dm < 8; ++dm) o[dm][nt][0] = o[dm][nt][1] = o[dm][nt][2] = o[dm][nt][3] = 0.f;
+        m_run[nt][0] = m_run[nt][1] = w_run[nt][0] = w_run[nt][1] = NEG_INF;
+        l_run[nt][0] = l_run[nt][1] = 0.f;
+        // q's B fragments: head 8 nt + gid, dims 16 kk + 4 tig .. + 3
+        const int head = 8 * nt + gid;
+        uint2 raw[8];
+        float top = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          raw[kk] = make_uint2(0u, 0u);
+          if (head < g)
+            raw[kk] = *reinterpret_cast<const uint2*>(sp + 2 * kDecode8TileBytes + head * 256 + kk * 32 + tig * 8);
+          top = fmaxf(top, fmaxf(fmaxf(fabsf(__uint_as_float(raw[kk].x << 16)),
+                                       fabsf(__uint_as_float(raw[kk].x & 0xffff0000u))),
+                                 fmaxf(fabsf(__uint_as_float(raw[kk].y << 16)),
+                                       fabsf(__uint_as_float(raw[kk].y & 0xffff0000u)))));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+        const float down = __uint_as_float((254u - e) << 23);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          qb[kk][nt][0] = pack_f16x2(__uint_as_float(raw[kk].x << 16) * down,
+                                     __uint_as_float(raw[kk].x & 0xffff0000u) * down);
+          qb[kk][nt][1] = pack_f16x2(__uint_as_float(raw[kk].y << 16) * down,
+                                     __uint_as_float(raw[kk].y & 0xffff0000u) * down);
+        }
+        const float up = __uint_as_float(e << 23) * p.scale_log2;
+        qs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * tig);
+        qs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * tig + 4);
+      }
+    }
+
+    const int tok_base = warp * 32;
+    if (tok_base < valid) {
+      const uint32_t sK = smem_u32(sp);
+      const uint32_t sV = sK + kDecode8TileBytes;
+      const int mi = lane >> 3;
+      const int lrow = tok_base + (mi & 1) * 8 + (lane & 7);
+      // ---- S^T = K Q^T: two 16-token tiles, 8 steps of 16 dims
+      float s[2][kNT][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
+#pragma unroll
+      for (int kp = 0; kp < 4; ++kp) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t r0, r1, r2, r3;  // tokens 0-7 / 8-15 of chunk 2 kp, then of 2 kp + 1
+          ldsm_x4(sK + swz128(lrow + 16 * mt, 2 * kp + (mi >> 1)), r0, r1, r2, r3);
+          const uint32_t a0 = e4m3x2_to_f16x2(r0), a2 = e4m3x2_hi_to_f16x2(r0);
+          const uint32_t a1 = e4m3x2_to_f16x2(r1), a3 = e4m3x2_hi_to_f16x2(r1);
+          const uint32_t c0 = e4m3x2_to_f16x2(r2), c2 = e4m3x2_hi_to_f16x2(r2);
+          const uint32_t c1 = e4m3x2_to_f16x2(r3), c3 = e4m3x2_hi_to_f16x2(r3);
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            mma_f16_16816(s[mt][nt], a0, a1, a2, a3, qb[2 * kp][nt][0], qb[2 * kp][nt][1]);
+            mma_f16_16816(s[mt][nt], c0, c1, c2, c3, qb[2 * kp + 1][nt][0], qb[2 * kp + 1][nt][1]);
+          }
+        }
+      }
+      // ---- scores in log2 units and the rows' V exponents
+      const bool partial = tok_base + 32 > valid;
+      float vk[2][2];
+      float ks[2][2];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int tk = tok_base + 16 * mt + 8 * r + gid;
+          ks[mt][r] = exp_byte_to_float(sexp[tk]);
+          vk[mt][r] = static_cast<float>(static_cast<int>(sexp[kDecode8Tile + tk]) - 127);
+        }
+      }
+      uint32_t wb[2][kNT][2];  // the weights as B fragments (two tokens of a head)
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        float mx[2] = {NEG_INF, NEG_INF}, wx[2] = {NEG_INF, NEG_INF};
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float v = s[mt][nt][c] * (ks[mt][c >> 1] * qs[nt][c & 1]);
+            if (partial && tok_base + 16 * mt + 8 * (c >> 1) + gid >= valid) v = NEG_INF;
+            s[mt][nt][c] = v;
+            mx[c & 1] = fmaxf(mx[c & 1], v);
+            wx[c & 1] = fmaxf(wx[c & 1], v + vk[mt][c >> 1]);
+          }
+        }
+        float m_use[2], w_use[2], w_scale[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+            wx[e] = fmaxf(wx[e], __shfl_xor_sync(0xffffffffu, wx[e], x));
+          }
+          const float m_new = fmaxf(m_run[nt][e], mx[e]);
+          const float w_new = fmaxf(w_run[nt][e], wx[e]);
+          m_use[e] = m_new == NEG_INF ? 0.f : m_new;
+          w_use[e] = w_new == NEG_INF ? 0.f : w_new;
+          l_run[nt][e] *= fast_exp2(m_run[nt][e] - m_use[e]);
+          w_scale[e] = fast_exp2(w_run[nt][e] - w_use[e]);
+          m_run[nt][e] = m_new;
+          w_run[nt][e] = w_new;
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          float w[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            l_run[nt][c & 1] += fast_exp2(s[mt][nt][c] - m_use[c & 1]);
+            w[c] = fast_exp2(s[mt][nt][c] + vk[mt][c >> 1] - w_use[c & 1]);
+          }
+          wb[mt][nt][0] = movmatrix_trans(pack_f16x2(w[0], w[1]));
+          wb[mt][nt][1] = movmatrix_trans(pack_f16x2(w[2], w[3]));
+        }
+#pragma unroll
+        for (int dm = 0; dm < 8; ++dm) {
+          o[dm][nt][0] *= w_scale[0];
+          o[dm][nt][1] *= w_scale[1];
+          o[dm][nt][2] *= w_scale[0];
+          o[dm][nt][3] *= w_scale[1];
+        }
+      }
+      // ---- O^T += V^T P^T: two steps of 16 tokens, 8 tiles of 16 dims
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;  // V of tokens past the end counts as 0
+        if (partial) {
+          const int tk = tok_base + 16 * mt + 2 * tig;
+          keep_lo = (tk < valid ? 0x0000ffffu : 0u) | (tk + 1 < valid ? 0xffff0000u : 0u);
+          keep_hi = (tk + 8 < valid ? 0x0000ffffu : 0u) | (tk + 9 < valid ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int dp = 0; dp < 4; ++dp) {
+          uint32_t r[4];  // tokens 0-7 / 8-15 of chunk 2 dp, then of 2 dp + 1
+          ldsm_x4_trans(sV + swz128(lrow + 16 * mt, 2 * dp + (mi >> 1)), r[0], r[1], r[2], r[3]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            // bytes: token 2 tig dims 2 gid, 2 gid + 1, token 2 tig + 1 the same
+            const uint32_t lo = __byte_perm(r[2 * half] & keep_lo, 0u, 0x3120);
+            const uint32_t hi = __byte_perm(r[2 * half + 1] & keep_hi, 0u, 0x3120);
+            const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_hi_to_f16x2(lo);
+            const uint32_t a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_hi_to_f16x2(hi);
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+              mma_f16_16816(o[2 * dp + half][nt], a0, a1, a2, a3, wb[mt][nt][0], wb[mt][nt][1]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&empty_bar[stage]));
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    if (!(flags & kLast)) continue;
+
+    // ---- the pair's tiles in this CTA are done: merge the four warps
+    float* st = state + (merges & 1u) * S::kStateFloats;
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float l = l_run[nt][e];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        const int head = 8 * nt + 2 * tig + e;
+        if (head < g) {
+          const float m = m_run[nt][e];
+          const float f = m == NEG_INF ? 0.f : fast_exp2(w_run[nt][e] - m);
+          float* dst = st + (warp * G + head) * kDecode8ORow;
+#pragma unroll
+          for (int dm = 0; dm < 8; ++dm)
+            *reinterpret_cast<float2*>(dst + 16 * dm + 2 * gid) =
+                make_float2(o[dm][nt][e] * f, o[dm][nt][2 + e] * f);
+          if (gid == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(m, l);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&merge_bar[merges & 1u]));
+    if (!mbar_wait_bounded(smem_u32(&merge_bar[merges & 1u]), (merges >> 1) & 1u)) {
+      *abort_flag = 1;
+      break;
+    }
+    ++merges;
+    for (int row = warp; row < g; row += kDecode8Warps) {
+      const float* src = st + row * kDecode8ORow;
+      float M = NEG_INF;
+#pragma unroll
+      for (int w = 0; w < kDecode8Warps; ++w) M = fmaxf(M, src[w * G * kDecode8ORow + 128]);
+      float L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kDecode8Warps; ++w) {
+        const float* ws = src + w * G * kDecode8ORow;
+        const float f = ws[128] == NEG_INF ? 0.f : fast_exp2(ws[128] - M);
+        const float4 x = *reinterpret_cast<const float4*>(ws + 4 * lane);
+        L += ws[129] * f;
+        acc.x += x.x * f;
+        acc.y += x.y * f;
+        acc.z += x.z * f;
+        acc.w += x.w * f;
+      }
+      if (!(flags & kPartial)) {
+        decode8_store(p.out + b * p.out_stride_token + (h * g + row) * 128 + 4 * lane, acc,
+                      L > 0.f ? 1.f / L : 0.f);
+      } else {
+        float* dst = p.parts + ((blockIdx.x * 2 + (flags & kPartialSlot1 ? 1 : 0)) * g + row) * kDecode8ORow;
+        *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
+        if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
+      }
+    }
+  }
+}
+
+// Joins the pieces of the pair that begins in CTA blockIdx.x's range and goes
+// on in later ones (head blockIdx.y of the group): each warp sums every eighth
+// piece, the first warp the eight sums, always in the same order.
+__global__ void __launch_bounds__(kDecode8JoinWarps * 32) decode_fp8_join_kernel(const Decode8Params p) {
+  __shared__ float sums[kDecode8JoinWarps][kDecode8ORow];
+  grid_dependency_wait();
+  allow_dependent_launch();
+  const Decode8Split split = p.splits[blockIdx.x];
+  if (split.pieces == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y;
+  // piece 0 is the range's last pair of this CTA, piece i the first of CTA + i
+  auto piece = [&](int i) {
+    return p.parts + ((static_cast<int>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * p.g + row) * kDecode8ORow;
+  };
+  float M = -INFINITY;
+  for (int i = warp + kDecode8JoinWarps * lane; i < split.pieces; i += kDecode8JoinWarps * 32)
+    M = fmaxf(M, piece(i)[128]);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = warp; i < split.pieces; i += kDecode8JoinWarps) {
+    const float* src = piece(i);
+    const float2 ml = *reinterpret_cast<const float2*>(src + 128);
+    const float4 x = *reinterpret_cast<const float4*>(src + 4 * lane);
+    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+    L += ml.y * f;
+    acc.x += x.x * f;
+    acc.y += x.y * f;
+    acc.z += x.z * f;
+    acc.w += x.w * f;
+  }
+  *reinterpret_cast<float4*>(&sums[warp][4 * lane]) = acc;
+  if (lane == 0) *reinterpret_cast<float2*>(&sums[warp][128]) = make_float2(M, L);
+  __syncthreads();
+  if (warp != 0) return;
+  M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kDecode8JoinWarps; ++w) M = fmaxf(M, sums[w][128]);
+  L = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < kDecode8JoinWarps; ++w) {
+    const float f = sums[w][128] == -INFINITY ? 0.f : fast_exp2(sums[w][128] - M);
+    const float4 x = *reinterpret_cast<const float4*>(&sums[w][4 * lane]);
+    L += sums[w][129] * f;
+    acc.x += x.x * f;
+    acc.y += x.y * f;
+    acc.z += x.z * f;
+    acc.w += x.w * f;
+  }
+  const int b = split.pair / p.num_kv_heads, h = split.pair - b * p.num_kv_heads;
+  decode8_store(p.out + b * p.out_stride_token + (h * p.g + row) * 128 + 4 * lane, acc,
+                L > 0.f ? 1.f / L : 0.f);
 }
 
 }  // namespace nkv
