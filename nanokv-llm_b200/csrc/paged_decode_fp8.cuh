@@ -9,8 +9,9 @@
 // FLOP, 2 g FLOP a byte.
 //
 // Split and join. The work of a call is the 128-token tiles of every (row, kv
-// head) pair in the order (row, head, tile); CTA c of n takes the tiles
-// [c T / n, (c + 1) T / n). Every CTA has the same number of tiles, whatever
+// head) pair in the order (head, row, tile); CTA c of n takes the tiles
+// [c T / n, (c + 1) T / n). (Heads outermost: CTAs n / Hk apart then read the
+// same tokens of different heads at the same time, neighbours in memory.) Every CTA has the same number of tiles, whatever
 // the lengths, and which tiles depends on the lengths alone: results are the
 // same every time. A CTA finishes the pairs that lie inside its range; of a
 // pair that it shares with others it leaves the raw (m, l, O) in the workspace
@@ -20,9 +21,9 @@
 //
 // One CTA per SM: a producer warp walks the range and keeps a ring of tiles
 // full (TMA for K and V, 128-byte rows, 128B swizzle; bulk copies for the
-// exponent bytes and the group's q rows), four consumer warps take 32 tokens
-// of every tile each, with a running softmax per warp that is merged in shared
-// memory at the end of a pair.
+// exponent bytes and the group's q rows), two groups of four consumer
+// warps take the tiles in turn, 32 tokens a warp, with a running softmax per
+// warp that is merged in shared memory at the end of a pair.
 //
 // Arithmetic. e4m3 is exact in f16, so K and V go to the tensor cores as f16
 // (mma.sync m16n8k16, 32-bit accumulators; groups of 1 to 16 heads are too
@@ -51,7 +52,7 @@
 namespace nkv {
 
 constexpr int kDecode8Tile = 128;
-constexpr int kDecode8Warps = 4;  // consumers
+constexpr int kDecode8Warps = 8;  // consumers: two groups of four, which take the tiles in turn
 constexpr int kDecode8Threads = (kDecode8Warps + 1) * 32;
 constexpr int kDecode8TileBytes = kDecode8Tile * 128;
 constexpr int kDecode8MaxCtas = 160;
@@ -67,7 +68,7 @@ struct Decode8Shape {
   // [K][V][q rows][K exponents][V exponents], 1024-byte aligned
   static constexpr int kStageBytes = 2 * kDecode8TileBytes + kQBytes + 1024;
   static constexpr int kStateFloats = kDecode8Warps * G * kDecode8ORow;
-  static constexpr int kBarOffset = kStages * kStageBytes + 2 * kStateFloats * 4;
+  static constexpr int kBarOffset = kStages * kStageBytes + kStateFloats * 4;
   static constexpr int kSmemBytes = kBarOffset + (2 * kStages + 2) * 8 + kStages * 16 + 16 + 1024;
 };
 
@@ -143,10 +144,10 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float* state = reinterpret_cast<float*>(smem + kStages * S::kStageBytes);  // two buffers
+  float* state = reinterpret_cast<float*>(smem + kStages * S::kStageBytes);  // the warps' (O, m, l)
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kBarOffset);
   uint64_t* empty_bar = full_bar + kStages;
-  uint64_t* merge_bar = empty_bar + kStages;  // one per state buffer
+  uint64_t* merge_bar = empty_bar + kStages;  // states written, states read
   // per stage: row (-1: no more tiles), head, flags | valid tokens << 8
   int* meta = reinterpret_cast<int*>(merge_bar + 2);
   volatile int* abort_flag = meta + kStages * 4;
@@ -190,6 +191,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     for (int b = lane; b < p.batch; b += 32) total += decode8_tiles(decode8_length(p, b));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int64_t head_tiles = total;
     total *= Hk;
     const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
     int64_t u = 0, left = 0;
@@ -197,42 +199,64 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       u = blockIdx.x * total / ctas;
       left = (blockIdx.x + 1) * total / ctas - u;
     }
-    // ---- its first row, head and tile
+    // the lengths of 32 rows from lens0, one per lane
+    int lens0 = 0, my_len = 0;
+    auto load_lengths = [&](int first) {
+      lens0 = first;
+      my_len = first + lane < p.batch ? decode8_length(p, first + lane) : 0;
+    };
+    // the first row with tokens at or after (head, row)
+    auto seek = [&](int& head, int& row) {
+      while (true) {
+        if (row >= p.batch) {
+          row = 0;
+          ++head;
+        }
+        if (row < lens0 || row >= lens0 + 32) load_lengths(row);
+        const unsigned some = __ballot_sync(0xffffffffu, my_len > 0) & (0xffffffffu << (row - lens0));
+        if (some != 0u) {
+          row = lens0 + __ffs(some) - 1;
+          return;
+        }
+        row = lens0 + 32;
+      }
+    };
+    // ---- its first head, row and tile
     int b = 0, h = 0, t = 0, len = 0, ntiles = 0;
     if (left > 0) {
-      int64_t base = 0;
-      for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int my_len = b0 + lane < p.batch ? decode8_length(p, b0 + lane) : 0;
-        const int my_tiles = decode8_tiles(my_len);
-        int64_t incl = my_tiles;
+      h = static_cast<int>(u / head_tiles);
+      int64_t rest = u - h * head_tiles;
+      for (int b0 = 0;; b0 += 32) {
+        load_lengths(b0);
+        int64_t incl = decode8_tiles(my_len);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
           if (lane >= o) incl += y;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, (base + incl) * Hk > u);
+        const unsigned past = __ballot_sync(0xffffffffu, incl > rest);
         if (past != 0u) {
           const int at = __ffs(past) - 1;
           b = b0 + at;
           len = __shfl_sync(0xffffffffu, my_len, at);
-          ntiles = __shfl_sync(0xffffffffu, my_tiles, at);
-          const int64_t rest = u - (base + __shfl_sync(0xffffffffu, incl, at) - ntiles) * Hk;
-          h = static_cast<int>(rest / ntiles);
-          t = static_cast<int>(rest - static_cast<int64_t>(h) * ntiles);
+          ntiles = decode8_tiles(len);
+          t = static_cast<int>(rest - (__shfl_sync(0xffffffffu, incl, at) - ntiles));
           break;
         }
-        base += __shfl_sync(0xffffffffu, incl, 31);
+        rest -= __shfl_sync(0xffffffffu, incl, 31);
       }
     }
-    // 32 entries of the row's block table from entry win0, one per lane
-    int win0 = 0, ent = -1;
-    auto load_window = [&](int first) {
-      win0 = first;
-      ent = -1;
-      if (first + lane < p.max_blocks)
-        ent = __ldg(p.block_tables + static_cast<int64_t>(b) * p.max_blocks + first + lane);
+    // 32 entries of a row's block table from entry `first`, one per lane
+    auto load_window = [&](int row, int first) {
+      return first + lane < p.max_blocks
+                 ? __ldg(p.block_tables + static_cast<int64_t>(row) * p.max_blocks + first + lane)
+                 : -1;
     };
-    if (left > 0) load_window(t * kDecode8Tile / p.block_size);
+    int win0 = 0, ent = -1;
+    if (left > 0) {
+      win0 = t * kDecode8Tile / p.block_size;
+      ent = load_window(b, win0);
+    }
     int stage = 0;
     uint32_t phase = 0;
     int64_t issued = 0;
@@ -248,13 +272,23 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         split.pair = b * Hk + h;
         split.pieces = static_cast<int>(((last_tile + 1) * ctas - 1) / total - blockIdx.x) + 1;
       }
+      // the next row: its length is at hand, its table entries are requested now
+      int next_h = h, next_b = b + 1, next_len = 0, next_ent = -1;
+      if (left > count) {
+        seek(next_h, next_b);
+        next_len = __shfl_sync(0xffffffffu, my_len, next_b - lens0);
+        next_ent = load_window(next_b, 0);
+      }
       for (int j = 0; j < count; ++j) {
         const int tok = (t + j) * kDecode8Tile;
         const int valid = min(kDecode8Tile, len - tok);
         const int page = tok / p.block_size;
         const int off = tok - page * p.block_size;  // 0 when pages are shorter than a tile
         const int pages = p.box_rows == kDecode8Tile ? 1 : (valid + p.box_rows - 1) / p.box_rows;
-        if (page + pages - 1 - win0 >= 32) load_window(page);
+        if (page + pages - 1 - win0 >= 32) {
+          win0 = page;
+          ent = load_window(b, page);
+        }
         const int blk = __shfl_sync(0xffffffffu, ent, (page - win0 + lane) & 31);
         const bool mine = lane < pages;
         const bool good = blk >= 0 && blk < p.num_blocks;
@@ -308,25 +342,12 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       u += count;
       left -= count;
       t = 0;
-      if (++h == Hk) {
-        h = 0;
-        // the next row that has tokens
-        while (left > 0) {
-          const int my = b + 1 + lane;
-          const int my_len = my < p.batch ? decode8_length(p, my) : 0;
-          const unsigned some = __ballot_sync(0xffffffffu, my_len > 0);
-          const int at = some != 0u ? __ffs(some) - 1 : 31;
-          b += 1 + at;
-          if (some != 0u) {
-            len = __shfl_sync(0xffffffffu, my_len, at);
-            ntiles = decode8_tiles(len);
-            break;
-          }
-        }
-        if (left > 0) load_window(0);
-      } else if (left > 0 && win0 != 0) {
-        load_window(0);
-      }
+      h = next_h;
+      b = next_b;
+      len = next_len;
+      ntiles = decode8_tiles(len);
+      win0 = 0;
+      ent = next_ent;
     }
     if (lane == 0) {
       p.splits[blockIdx.x] = split;
@@ -361,6 +382,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   int stage = 0;
   uint32_t phase = 0;
   uint32_t merges = 0;
+  uint32_t turn = warp >> 2;  // even: the tile is this group's
   while (true) {
     if (!mbar_wait_bounded(smem_u32(&full_bar[stage]), phase)) {
       *abort_flag = 1;
@@ -412,8 +434,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       }
     }
 
-    const int tok_base = warp * 32;
-    if (tok_base < valid) {
+    const int tok_base = (warp & 3) * 32;
+    if ((turn++ & 1u) == 0u && tok_base < valid) {
       const uint32_t sK = smem_u32(sp);
       const uint32_t sV = sK + kDecode8TileBytes;
       const int mi = lane >> 3;
@@ -540,8 +562,11 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     }
     if (!(flags & kLast)) continue;
 
-    // ---- the pair's tiles in this CTA are done: merge the four warps
-    float* st = state + (merges & 1u) * S::kStateFloats;
+    // ---- the pair's tiles in this CTA are done: merge the warps
+    if (!mbar_wait_bounded(smem_u32(&merge_bar[1]), (merges & 1u) ^ 1u)) {
+      *abort_flag = 1;
+      break;
+    }
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
@@ -553,7 +578,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         if (head < g) {
           const float m = m_run[nt][e];
           const float f = m == NEG_INF ? 0.f : fast_exp2(w_run[nt][e] - m);
-          float* dst = st + (warp * G + head) * kDecode8ORow;
+          float* dst = state + (warp * G + head) * kDecode8ORow;
 #pragma unroll
           for (int dm = 0; dm < 8; ++dm)
             *reinterpret_cast<float2*>(dst + 16 * dm + 2 * gid) =
@@ -563,14 +588,14 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&merge_bar[merges & 1u]));
-    if (!mbar_wait_bounded(smem_u32(&merge_bar[merges & 1u]), (merges >> 1) & 1u)) {
+    if (lane == 0) mbar_arrive(smem_u32(&merge_bar[0]));
+    if (!mbar_wait_bounded(smem_u32(&merge_bar[0]), merges & 1u)) {
       *abort_flag = 1;
       break;
     }
     ++merges;
     for (int row = warp; row < g; row += kDecode8Warps) {
-      const float* src = st + row * kDecode8ORow;
+      const float* src = state + row * kDecode8ORow;
       float M = NEG_INF;
 #pragma unroll
       for (int w = 0; w < kDecode8Warps; ++w) M = fmaxf(M, src[w * G * kDecode8ORow + 128]);
@@ -596,6 +621,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&merge_bar[1]));
   }
 }
 
