@@ -19,7 +19,7 @@
 // behind the first with programmatic dependence, joins in the CTAs' order. No
 // counters, so the workspace needs no content and outlives nothing.
 //
-// One CTA per SM: a producer warp walks the range and keeps a ring of tiles
+// One CTA per SM: two producer warps walk the range and keep a ring of tiles
 // full (TMA for K and V, 128-byte rows, 128B swizzle; bulk copies for the
 // exponent bytes and the group's q rows), two groups of four consumer
 // warps take the tiles in turn, 32 tokens a warp, with a running softmax per
@@ -53,7 +53,7 @@ namespace nkv {
 
 constexpr int kDecode8Tile = 128;
 constexpr int kDecode8Warps = 8;  // consumers: two groups of four, which take the tiles in turn
-constexpr int kDecode8Threads = (kDecode8Warps + 1) * 32;
+constexpr int kDecode8Threads = (kDecode8Warps + 2) * 32;  // and two producers, K's and V's
 constexpr int kDecode8TileBytes = kDecode8Tile * 128;
 constexpr int kDecode8MaxCtas = 160;
 constexpr int kDecode8ORow = 132;   // floats of one row of a partial: O[128], m, l, 2 of padding
@@ -63,7 +63,7 @@ template <int G>
 struct Decode8Shape {
   static_assert(G == 1 || G == 2 || G == 4 || G == 8 || G == 16, "padded group width");
   static constexpr int kNT = G <= 8 ? 1 : 2;  // 8-head column tiles
-  static constexpr int kStages = G <= 8 ? 5 : 4;
+  static constexpr int kStages = G <= 4 ? 6 : G <= 8 ? 5 : 4;
   static constexpr int kQBytes = (G < 4 ? 4 : G) * 256;
   // [K][V][q rows][K exponents][V exponents], 1024-byte aligned
   static constexpr int kStageBytes = 2 * kDecode8TileBytes + kQBytes + 1024;
@@ -101,7 +101,7 @@ struct Decode8Params {
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                               uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(  // registers only: left to the compiler to schedule
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
       "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -157,7 +157,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&full_bar[s]), 2);
       mbar_init(smem_u32(&empty_bar[s]), kDecode8Warps);
     }
     mbar_init(smem_u32(&merge_bar[0]), kDecode8Warps);
@@ -182,10 +182,22 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int Hk = p.num_kv_heads;
   const int g = p.g;
 
-  if (warp == kDecode8Warps) {
-    // ------------------------------------------------------------ producer
+  if (warp >= kDecode8Warps) {
+    // ----------------------------------------------------------- producers
+    // Both walk the same tiles; one copies K, its exponents and q, the other V
+    // and its exponents. A lane holds the position of one box (min(block_size,
+    // 128) tokens) of the 32 ahead and issues that box's copies itself, so a
+    // tile costs no division, shuffle or table load.
+    const bool for_k = warp == kDecode8Warps;
+    const CUtensorMap* tm = for_k ? &tm_k : &tm_v;
+    const uint8_t* exps = for_k ? p.k_exp : p.v_exp;
+    const uint32_t value_off = for_k ? 0u : static_cast<uint32_t>(kDecode8TileBytes);
+    const uint32_t exp_off = 2 * kDecode8TileBytes + S::kQBytes + (for_k ? 0u : static_cast<uint32_t>(kDecode8Tile));
     const uint64_t policy = l2_policy_evict_first();
-    const uint32_t q_bytes = static_cast<uint32_t>(g) * 256u;
+    const uint32_t q_bytes = for_k ? static_cast<uint32_t>(g) * 256u : 0u;
+    const int box_shift = 31 - __clz(p.box_rows);
+    const int tile_boxes = kDecode8Tile >> box_shift;
+    const int page_boxes = p.block_size >> box_shift;
     // ---- this CTA's range of tiles
     int64_t total = 0;
     for (int b = lane; b < p.batch; b += 32) total += decode8_tiles(decode8_length(p, b));
@@ -246,28 +258,45 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         rest -= __shfl_sync(0xffffffffu, incl, 31);
       }
     }
-    // 32 entries of a row's block table from entry `first`, one per lane
-    auto load_window = [&](int row, int first) {
-      return first + lane < p.max_blocks
-                 ? __ldg(p.block_tables + static_cast<int64_t>(row) * p.max_blocks + first + lane)
+    // the table entry of this lane's box, first + lane, of a row
+    auto load_entry = [&](int row, int first) {
+      const int page = (first + lane) / page_boxes;
+      return page < p.max_blocks
+                 ? __ldg(p.block_tables + static_cast<int64_t>(row) * p.max_blocks + page)
                  : -1;
     };
-    int win0 = 0, ent = -1;
-    if (left > 0) {
-      win0 = t * kDecode8Tile / p.block_size;
-      ent = load_window(b, win0);
-    }
+    int box0 = 0, slot = 0;   // the window's first box; this lane's box's first slot
+    const uint8_t* exp_src = exps;
+    unsigned good = 0u;       // the window's boxes that have a page
+    auto set_window = [&](int first, int blk) {
+      box0 = first;
+      const bool ok = blk >= 0 && blk < p.num_blocks;
+      const int off = ((first + lane) % page_boxes) << box_shift;
+      // no page: rows far outside the tensor, which TMA fills with zeros
+      slot = ok ? blk * p.block_size + off : -2 * kDecode8Tile;
+      exp_src = exps + (static_cast<int64_t>(blk) * Hk + h) * p.block_size + off;
+      good = __ballot_sync(0xffffffffu, ok);
+    };
+    if (left > 0) set_window(t * tile_boxes, load_entry(b, t * tile_boxes));
     int stage = 0;
     uint32_t phase = 0;
     int64_t issued = 0;
     bool ok = true;
+    auto wait_empty = [&]() {
+      const uint32_t bar = smem_u32(&empty_bar[stage]);
+      for (uint32_t i = 0; i < kWaitPollLimit; ++i) {
+        if (mbar_try_wait(bar, phase ^ 1u)) return true;
+        if (*abort_flag != 0) return false;
+      }
+      raise_error(NKV_DEVERR_WAIT_TIMEOUT);
+      return false;
+    };
     Decode8Split split{0, 0};
     while (left > 0 && ok) {
       // ---- tiles [t, t + count) of (b, h)
       const int count = static_cast<int>(min(left, static_cast<int64_t>(ntiles - t)));
-      const bool whole = count == ntiles;
-      const bool begins = t == 0;
-      if (begins && !whole) {
+      const int seg_flags = (count == ntiles ? 0 : kPartial) | (t == 0 ? kPartialSlot1 : 0);
+      if (t == 0 && count != ntiles) {
         const int64_t last_tile = u + ntiles - 1;
         split.pair = b * Hk + h;
         split.pieces = static_cast<int>(((last_tile + 1) * ctas - 1) / total - blockIdx.x) + 1;
@@ -277,62 +306,54 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       if (left > count) {
         seek(next_h, next_b);
         next_len = __shfl_sync(0xffffffffu, my_len, next_b - lens0);
-        next_ent = load_window(next_b, 0);
+        next_ent = load_entry(next_b, 0);
       }
       for (int j = 0; j < count; ++j) {
-        const int tok = (t + j) * kDecode8Tile;
-        const int valid = min(kDecode8Tile, len - tok);
-        const int page = tok / p.block_size;
-        const int off = tok - page * p.block_size;  // 0 when pages are shorter than a tile
-        const int pages = p.box_rows == kDecode8Tile ? 1 : (valid + p.box_rows - 1) / p.box_rows;
-        if (page + pages - 1 - win0 >= 32) {
-          win0 = page;
-          ent = load_window(b, page);
+        int first = (t + j) * tile_boxes - box0;  // the tile's first box within the window
+        if (first >= 32) {
+          set_window(box0 + first, load_entry(b, box0 + first));
+          first = 0;
         }
-        const int blk = __shfl_sync(0xffffffffu, ent, (page - win0 + lane) & 31);
-        const bool mine = lane < pages;
-        const bool good = blk >= 0 && blk < p.num_blocks;
-        const unsigned good_pages = __ballot_sync(0xffffffffu, mine && good);
-        if (mine && !good) raise_error(NKV_DEVERR_DECODE_BLOCK);
-        if (lane == 0) ok = *abort_flag == 0 && mbar_wait_bounded(smem_u32(&empty_bar[stage]), phase ^ 1u);
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        const int valid = min(kDecode8Tile, len - (t + j) * kDecode8Tile);
+        const int boxes = (valid + p.box_rows - 1) >> box_shift;
+        const int at = lane - first;
+        if (at >= 0 && at < boxes) {
+          ok = wait_empty();
+          if (ok) {
+            const uint32_t sbase = smem_u32(smem + stage * S::kStageBytes);
+            const uint32_t bar = smem_u32(&full_bar[stage]);
+            if (at == 0) {
+              if (for_k) {
+                int* m = meta + stage * 4;
+                m[0] = b;
+                m[1] = h;
+                m[2] = seg_flags | (j == 0 ? kFirst : 0) | (j == count - 1 ? kLast : 0) | (valid << 8);
+              }
+              const unsigned with_exps = (good >> first) & (0xffu >> (8 - boxes));
+              mbar_arrive_expect_tx(bar, ((boxes * 128u + __popc(with_exps)) << box_shift) +
+                                             (j == 0 ? q_bytes : 0u));
+              if (for_k && j == 0) {
+                const __nv_bfloat16* src =
+                    p.q + b * p.q_stride_token + static_cast<int64_t>(h) * g * p.q_stride_head;
+                const uint32_t sq = sbase + 2 * kDecode8TileBytes;
+                if (p.q_stride_head == 128) {
+                  bulk_load_row(sq, src, q_bytes, bar);
+                } else {
+                  for (int r = 0; r < g; ++r) bulk_load_row(sq + r * 256, src + r * p.q_stride_head, 256, bar);
+                }
+              }
+            }
+            tma_load_3d(sbase + value_off + (static_cast<uint32_t>(at * 128) << box_shift), tm, bar, 0, h, slot,
+                        policy);
+            if ((good >> lane) & 1u) {
+              bulk_load_row(sbase + exp_off + (at << box_shift), exp_src, p.box_rows, bar);
+            } else {
+              raise_error(NKV_DEVERR_DECODE_BLOCK);
+            }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok) != 0;
         if (!ok) break;
-        uint8_t* sp = smem + stage * S::kStageBytes;
-        const uint32_t sbase = smem_u32(sp);
-        const uint32_t bar = smem_u32(&full_bar[stage]);
-        if (lane == 0) {
-          int* m = meta + stage * 4;
-          m[0] = b;
-          m[1] = h;
-          m[2] = (j == 0 ? kFirst : 0) | (j == count - 1 ? kLast : 0) | (whole ? 0 : kPartial) |
-                 (begins ? kPartialSlot1 : 0) | (valid << 8);
-          mbar_arrive_expect_tx(bar, static_cast<uint32_t>(pages * p.box_rows * 256) +
-                                         __popc(good_pages) * p.box_rows * 2 +
-                                         (j == 0 ? q_bytes : 0u));
-        }
-        __syncwarp();
-        if (mine) {
-          // a page that is none: rows far outside the tensor, which TMA fills with zeros
-          const int row = good ? blk * p.block_size + off : -2 * kDecode8Tile;
-          const uint32_t at = static_cast<uint32_t>(lane * p.box_rows);
-          tma_load_3d(sbase + at * 128u, &tm_k, bar, 0, h, row, policy);
-          tma_load_3d(sbase + kDecode8TileBytes + at * 128u, &tm_v, bar, 0, h, row, policy);
-          if (good) {
-            const int64_t e = (static_cast<int64_t>(blk) * Hk + h) * p.block_size + off;
-            const uint32_t se = sbase + 2 * kDecode8TileBytes + S::kQBytes + at;
-            bulk_load_row(se, p.k_exp + e, p.box_rows, bar);
-            bulk_load_row(se + kDecode8Tile, p.v_exp + e, p.box_rows, bar);
-          }
-        }
-        if (j == 0) {
-          const __nv_bfloat16* src = p.q + b * p.q_stride_token + static_cast<int64_t>(h) * g * p.q_stride_head;
-          const uint32_t sq = sbase + 2 * kDecode8TileBytes;
-          if (p.q_stride_head == 128) {
-            if (lane == 0) bulk_load_row(sq, src, q_bytes, bar);
-          } else if (lane < g) {
-            bulk_load_row(sq + lane * 256, src + lane * p.q_stride_head, 256, bar);
-          }
-        }
         ++issued;
         if (++stage == kStages) {
           stage = 0;
@@ -346,13 +367,12 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       b = next_b;
       len = next_len;
       ntiles = decode8_tiles(len);
-      win0 = 0;
-      ent = next_ent;
+      set_window(0, next_ent);
     }
     if (lane == 0) {
-      p.splits[blockIdx.x] = split;
-      if (ok && mbar_wait_bounded(smem_u32(&empty_bar[stage]), phase ^ 1u)) {
-        meta[stage * 4] = -1;
+      if (for_k) p.splits[blockIdx.x] = split;
+      if (ok && wait_empty()) {
+        if (for_k) meta[stage * 4] = -1;
         mbar_arrive(smem_u32(&full_bar[stage]));
       } else {
         *abort_flag = 1;
@@ -440,30 +460,41 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       const uint32_t sV = sK + kDecode8TileBytes;
       const int mi = lane >> 3;
       const int lrow = tok_base + (mi & 1) * 8 + (lane & 7);
-      // ---- S^T = K Q^T: two 16-token tiles, 8 steps of 16 dims
-      float s[2][kNT][4];
+      // ---- S^T = K Q^T: two 16-token tiles, 8 steps of 16 dims. All loads first
+      // (each waits for none of the others), even and odd pairs of steps in
+      // sums of their own.
+      uint32_t raw[2][4][4];  // [token tile][pair of 16-byte chunks]: tokens 0-7 / 8-15 of the first, of the second
+#pragma unroll
+      for (int kp = 0; kp < 4; ++kp)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+          ldsm_x4(sK + swz128(lrow + 16 * mt, 2 * kp + (mi >> 1)), raw[mt][kp][0], raw[mt][kp][1],
+                  raw[mt][kp][2], raw[mt][kp][3]);
+      float s[2][kNT][4], s_odd[2][kNT][4];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[mt][nt][c] = s_odd[mt][nt][c] = 0.f;
 #pragma unroll
       for (int kp = 0; kp < 4; ++kp) {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-          uint32_t r0, r1, r2, r3;  // tokens 0-7 / 8-15 of chunk 2 kp, then of 2 kp + 1
-          ldsm_x4(sK + swz128(lrow + 16 * mt, 2 * kp + (mi >> 1)), r0, r1, r2, r3);
-          const uint32_t a0 = e4m3x2_to_f16x2(r0), a2 = e4m3x2_hi_to_f16x2(r0);
-          const uint32_t a1 = e4m3x2_to_f16x2(r1), a3 = e4m3x2_hi_to_f16x2(r1);
-          const uint32_t c0 = e4m3x2_to_f16x2(r2), c2 = e4m3x2_hi_to_f16x2(r2);
-          const uint32_t c1 = e4m3x2_to_f16x2(r3), c3 = e4m3x2_hi_to_f16x2(r3);
+          const uint32_t(&r)[4] = raw[mt][kp];
+          const uint32_t a0 = e4m3x2_to_f16x2(r[0]), a2 = e4m3x2_hi_to_f16x2(r[0]);
+          const uint32_t a1 = e4m3x2_to_f16x2(r[1]), a3 = e4m3x2_hi_to_f16x2(r[1]);
+          const uint32_t c0 = e4m3x2_to_f16x2(r[2]), c2 = e4m3x2_hi_to_f16x2(r[2]);
+          const uint32_t c1 = e4m3x2_to_f16x2(r[3]), c3 = e4m3x2_hi_to_f16x2(r[3]);
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) {
             mma_f16_16816(s[mt][nt], a0, a1, a2, a3, qb[2 * kp][nt][0], qb[2 * kp][nt][1]);
-            mma_f16_16816(s[mt][nt], c0, c1, c2, c3, qb[2 * kp + 1][nt][0], qb[2 * kp + 1][nt][1]);
+            mma_f16_16816(s_odd[mt][nt], c0, c1, c2, c3, qb[2 * kp + 1][nt][0], qb[2 * kp + 1][nt][1]);
           }
         }
       }
-      // ---- scores in log2 units and the rows' V exponents
+      // ---- the rest of the tile into registers, then the stage goes back to the
+      // producer: what a warp holds of the ring is not in flight from memory
       const bool partial = tok_base + 32 > valid;
       float vk[2][2];
       float ks[2][2];
@@ -476,6 +507,15 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
           vk[mt][r] = static_cast<float>(static_cast<int>(sexp[kDecode8Tile + tk]) - 127);
         }
       }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int dp = 0; dp < 4; ++dp)
+          ldsm_x4_trans(sV + swz128(lrow + 16 * mt, 2 * dp + (mi >> 1)), raw[mt][dp][0], raw[mt][dp][1],
+                        raw[mt][dp][2], raw[mt][dp][3]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&empty_bar[stage]));
+      // ---- scores in log2 units, weights
       uint32_t wb[2][kNT][2];  // the weights as B fragments (two tokens of a head)
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
@@ -484,7 +524,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            float v = s[mt][nt][c] * (ks[mt][c >> 1] * qs[nt][c & 1]);
+            float v = (s[mt][nt][c] + s_odd[mt][nt][c]) * (ks[mt][c >> 1] * qs[nt][c & 1]);
             if (partial && tok_base + 16 * mt + 8 * (c >> 1) + gid >= valid) v = NEG_INF;
             s[mt][nt][c] = v;
             mx[c & 1] = fmaxf(mx[c & 1], v);
@@ -538,8 +578,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         }
 #pragma unroll
         for (int dp = 0; dp < 4; ++dp) {
-          uint32_t r[4];  // tokens 0-7 / 8-15 of chunk 2 dp, then of 2 dp + 1
-          ldsm_x4_trans(sV + swz128(lrow + 16 * mt, 2 * dp + (mi >> 1)), r[0], r[1], r[2], r[3]);
+          const uint32_t(&r)[4] = raw[mt][dp];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             // bytes: token 2 tig dims 2 gid, 2 gid + 1, token 2 tig + 1 the same
@@ -553,9 +592,10 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
           }
         }
       }
+    } else {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&empty_bar[stage]));
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&empty_bar[stage]));
     if (++stage == kStages) {
       stage = 0;
       phase ^= 1u;
