@@ -19,6 +19,10 @@
 // behind the first with programmatic dependence, joins in the CTAs' order. No
 // counters, so the workspace needs no content and outlives nothing.
 //
+// Small calls, whose time is latency, are launched as thread-block clusters
+// instead, one per (row, kv head): no scan of the lengths, and the CTAs' parts
+// are joined through distributed shared memory by the same kernel.
+//
 // One CTA per SM: two producer warps walk the range and keep a ring of tiles
 // full (TMA for K and V, 128-byte rows, 128B swizzle; bulk copies for the
 // exponent bytes and the group's q rows), two groups of four consumer
@@ -58,6 +62,7 @@ constexpr int kDecode8TileBytes = kDecode8Tile * 128;
 constexpr int kDecode8MaxCtas = 160;
 constexpr int kDecode8ORow = 132;   // floats of one row of a partial: O[128], m, l, 2 of padding
 constexpr int kDecode8JoinWarps = 8;
+constexpr int kDecode8MaxCluster = 8;
 
 template <int G>
 struct Decode8Shape {
@@ -95,6 +100,7 @@ struct Decode8Params {
   float scale_log2;
   __nv_bfloat16* out;
   int64_t out_stride_token;
+  int cluster;           // > 1: clusters of that many CTAs, one per (row, kv head), that join by themselves
   Decode8Split* splits;  // [CTAs]
   float* parts;          // [CTAs][2][g][kDecode8ORow]: range's first pair, last pair
 };
@@ -111,6 +117,20 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
 }
 
 // Length of row b, kept inside its block table.
@@ -134,7 +154,9 @@ __device__ __forceinline__ void decode8_store(__nv_bfloat16* dst, float4 v, floa
   *reinterpret_cast<uint2*>(dst) = u;
 }
 
-template <int G>
+// kCluster: launched as clusters of p.cluster CTAs, one per (row, kv head). (A
+// kernel of its own: the join's code in the split form cost it 3 %.)
+template <int G, bool kCluster>
 __global__ void __launch_bounds__(kDecode8Threads, 1)
 paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const Decode8Params p) {
@@ -179,6 +201,11 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   grid_dependency_wait();
   allow_dependent_launch();
 
+  const int csize = p.cluster;
+  if (kCluster && static_cast<int>(cluster_nctarank()) != csize) {
+    if (threadIdx.x == 0) raise_error(NKV_DEVERR_LAUNCH_SHAPE);
+    return;
+  }
   const int Hk = p.num_kv_heads;
   const int g = p.g;
 
@@ -199,17 +226,26 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     const int tile_boxes = kDecode8Tile >> box_shift;
     const int page_boxes = p.block_size >> box_shift;
     // ---- this CTA's range of tiles
-    int64_t total = 0;
-    for (int b = lane; b < p.batch; b += 32) total += decode8_tiles(decode8_length(p, b));
+    int b = 0, h = 0, t = 0, len = 0, ntiles = 0;
+    int64_t u = 0, left = 0, total = 0, ctas = 1, head_tiles = 0;
+    if (kCluster) {
+      const int pair = static_cast<int>(blockIdx.x) / csize, rank = static_cast<int>(blockIdx.x) % csize;
+      b = pair / Hk;
+      h = pair - b * Hk;
+      len = decode8_length(p, b);
+      ntiles = decode8_tiles(len);
+      t = rank * ntiles / csize;
+      left = (rank + 1) * ntiles / csize - t;
+    } else {
+      for (int i = lane; i < p.batch; i += 32) head_tiles += decode8_tiles(decode8_length(p, i));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int64_t head_tiles = total;
-    total *= Hk;
-    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
-    int64_t u = 0, left = 0;
-    if (static_cast<int64_t>(blockIdx.x) < ctas) {
-      u = blockIdx.x * total / ctas;
-      left = (blockIdx.x + 1) * total / ctas - u;
+      for (int o = 16; o > 0; o >>= 1) head_tiles += __shfl_xor_sync(0xffffffffu, head_tiles, o);
+      total = head_tiles * Hk;
+      ctas = min(static_cast<int64_t>(gridDim.x), total);
+      if (static_cast<int64_t>(blockIdx.x) < ctas) {
+        u = blockIdx.x * total / ctas;
+        left = (blockIdx.x + 1) * total / ctas - u;
+      }
     }
     // the lengths of 32 rows from lens0, one per lane
     int lens0 = 0, my_len = 0;
@@ -234,8 +270,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       }
     };
     // ---- its first head, row and tile
-    int b = 0, h = 0, t = 0, len = 0, ntiles = 0;
-    if (left > 0) {
+    if (!kCluster && left > 0) {
       h = static_cast<int>(u / head_tiles);
       int64_t rest = u - h * head_tiles;
       for (int b0 = 0;; b0 += 32) {
@@ -296,7 +331,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       // ---- tiles [t, t + count) of (b, h)
       const int count = static_cast<int>(min(left, static_cast<int64_t>(ntiles - t)));
       const int seg_flags = (count == ntiles ? 0 : kPartial) | (t == 0 ? kPartialSlot1 : 0);
-      if (t == 0 && count != ntiles) {
+      if (!kCluster && t == 0 && count != ntiles) {
         const int64_t last_tile = u + ntiles - 1;
         split.pair = b * Hk + h;
         split.pieces = static_cast<int>(((last_tile + 1) * ctas - 1) / total - blockIdx.x) + 1;
@@ -370,7 +405,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       set_window(0, next_ent);
     }
     if (lane == 0) {
-      if (for_k) p.splits[blockIdx.x] = split;
+      if (for_k && !kCluster) p.splits[blockIdx.x] = split;
       if (ok && wait_empty()) {
         if (for_k) meta[stage * 4] = -1;
         mbar_arrive(smem_u32(&full_bar[stage]));
@@ -389,7 +424,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int tig = lane & 3;
   const float NEG_INF = -INFINITY;
   // rows without a token
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+  for (int b = blockIdx.x; !kCluster && b < p.batch; b += gridDim.x) {
     if (__ldg(p.context_lens + b) > 0 && p.max_blocks > 0) continue;
     uint4* dst = reinterpret_cast<uint4*>(p.out + b * p.out_stride_token);
     for (int i = threadIdx.x; i < Hk * g * 16; i += kDecode8Warps * 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -652,7 +687,12 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         acc.z += x.z * f;
         acc.w += x.w * f;
       }
-      if (!(flags & kPartial)) {
+      if (kCluster) {
+        // every tile of this CTA is consumed: the ring's memory is free
+        float* dst = reinterpret_cast<float*>(smem) + row * kDecode8ORow;
+        *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
+        if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
+      } else if (!(flags & kPartial)) {
         decode8_store(p.out + b * p.out_stride_token + (h * g + row) * 128 + 4 * lane, acc,
                       L > 0.f ? 1.f / L : 0.f);
       } else {
@@ -664,6 +704,53 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&merge_bar[1]));
   }
+  if constexpr (!kCluster) return;
+
+  // ---- cluster launch: the CTAs' rows are joined through distributed shared
+  // memory, in rank order, each CTA taking some of the group's heads
+  const int rank = static_cast<int>(blockIdx.x) % csize;
+  const int pair = static_cast<int>(blockIdx.x) / csize;
+  if (merges == 0) {  // no tile fell to this CTA
+    for (int row = warp; row < g; row += kDecode8Warps) {
+      float* dst = reinterpret_cast<float*>(smem) + row * kDecode8ORow;
+      *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(NEG_INF, 0.f);
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();
+  const int row = warp * csize + rank;
+  if (row < g) {
+    float4 x[kDecode8MaxCluster];
+    float2 ml[kDecode8MaxCluster];
+    float M = NEG_INF;
+#pragma unroll
+    for (int c = 0; c < kDecode8MaxCluster; ++c) {
+      ml[c] = make_float2(NEG_INF, 0.f);
+      x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < csize) {
+        const uint32_t src = mapa_shared(smem_u32(smem) + row * kDecode8ORow * 4, c);
+        x[c] = ld_cluster_f32x4(src + 16 * lane);
+        ml[c] = ld_cluster_f32x2(src + 512);
+        M = fmaxf(M, ml[c].x);
+      }
+    }
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < kDecode8MaxCluster; ++c) {
+      const float f = ml[c].x == NEG_INF ? 0.f : fast_exp2(ml[c].x - M);
+      L += ml[c].y * f;
+      acc.x += x[c].x * f;
+      acc.y += x[c].y * f;
+      acc.z += x[c].z * f;
+      acc.w += x[c].w * f;
+    }
+    decode8_store(p.out + (pair / Hk) * p.out_stride_token + ((pair % Hk) * g + row) * 128 + 4 * lane, acc,
+                  L > 0.f ? 1.f / L : 0.f);
+  }
+  __syncwarp();
+  cluster_sync_all();  // no CTA leaves while another reads its rows
 }
 
 // Joins the pieces of the pair that begins in CTA blockIdx.x's range and goes
