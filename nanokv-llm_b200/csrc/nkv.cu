@@ -1363,7 +1363,7 @@ int launch_decode8(const CUtensorMap& tk, const CUtensorMap& tv, nkv::Decode8Par
     attr_set[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(nkv::kDecode8Threads);
+  cfg.blockDim = dim3(nkv::kDecode8Threads<true>);
   cfg.dynamicSmemBytes = S::kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -1391,6 +1391,7 @@ int launch_decode8(const CUtensorMap& tk, const CUtensorMap& tv, nkv::Decode8Par
   *joined = p.cluster > 1;
   if (*joined) return cuda_status(cudaLaunchKernelEx(&cfg, cluster, tk, tv, p));
   cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(nkv::kDecode8Threads<false>);
   cfg.numAttrs = 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, split, tk, tv, p));
 }

@@ -27,7 +27,7 @@
 // full (TMA for K and V, 128-byte rows, 128B swizzle; bulk copies for the
 // exponent bytes and the group's q rows), two groups of four consumer
 // warps take the tiles in turn, 32 tokens a warp, with a running softmax per
-// warp that is merged in shared memory at the end of a pair.
+// warp; at the end of a pair a merger warp joins their states while they go on.
 //
 // Arithmetic. e4m3 is exact in f16, so K and V go to the tensor cores as f16
 // (mma.sync m16n8k16, 32-bit accumulators; groups of 1 to 16 heads are too
@@ -57,7 +57,9 @@ namespace nkv {
 
 constexpr int kDecode8Tile = 128;
 constexpr int kDecode8Warps = 8;  // consumers: two groups of four, which take the tiles in turn
-constexpr int kDecode8Threads = (kDecode8Warps + 2) * 32;  // and two producers, K's and V's
+constexpr int kDecode8Merger = kDecode8Warps + 2;  // after two producers, K's and V's
+template <bool kCluster>
+constexpr int kDecode8Threads = (kDecode8Merger + (kCluster ? 0 : 1)) * 32;
 constexpr int kDecode8TileBytes = kDecode8Tile * 128;
 constexpr int kDecode8MaxCtas = 160;
 constexpr int kDecode8ORow = 132;   // floats of one row of a partial: O[128], m, l, 2 of padding
@@ -72,9 +74,11 @@ struct Decode8Shape {
   static constexpr int kQBytes = (G < 4 ? 4 : G) * 256;
   // [K][V][q rows][K exponents][V exponents], 1024-byte aligned
   static constexpr int kStageBytes = 2 * kDecode8TileBytes + kQBytes + 1024;
+  // the warps' (O, m, l) of a pair, as many pairs as fit beside the ring
   static constexpr int kStateFloats = kDecode8Warps * G * kDecode8ORow;
-  static constexpr int kBarOffset = kStages * kStageBytes + kStateFloats * 4;
-  static constexpr int kSmemBytes = kBarOffset + (2 * kStages + 2) * 8 + kStages * 16 + 16 + 1024;
+  static constexpr int kSlots = G <= 2 ? 2 : 1;
+  static constexpr int kBarOffset = kStages * kStageBytes + kSlots * kStateFloats * 4;
+  static constexpr int kSmemBytes = kBarOffset + (2 * kStages + 2 * kSlots) * 8 + kStages * 16 + kSlots * 16 + 16 + 1024;
 };
 
 // What CTA c leaves for the join: the pair that begins in its range and goes
@@ -157,7 +161,7 @@ __device__ __forceinline__ void decode8_store(__nv_bfloat16* dst, float4 v, floa
 // kCluster: launched as clusters of p.cluster CTAs, one per (row, kv head). (A
 // kernel of its own: the join's code in the split form cost it 3 %.)
 template <int G, bool kCluster>
-__global__ void __launch_bounds__(kDecode8Threads, 1)
+__global__ void __launch_bounds__(kDecode8Threads<kCluster>, 1)
 paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const Decode8Params p) {
   using S = Decode8Shape<G>;
@@ -166,13 +170,16 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float* state = reinterpret_cast<float*>(smem + kStages * S::kStageBytes);  // the warps' (O, m, l)
+  constexpr int kSlots = S::kSlots;
+  float* state = reinterpret_cast<float*>(smem + kStages * S::kStageBytes);  // [slots]
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kBarOffset);
   uint64_t* empty_bar = full_bar + kStages;
-  uint64_t* merge_bar = empty_bar + kStages;  // states written, states read
-  // per stage: row (-1: no more tiles), head, flags | valid tokens << 8
-  int* meta = reinterpret_cast<int*>(merge_bar + 2);
-  volatile int* abort_flag = meta + kStages * 4;
+  uint64_t* state_full = empty_bar + kStages;  // per slot: written by all consumer warps
+  uint64_t* state_empty = state_full + kSlots;  // and read again
+  // per stage: row (-1: no more tiles), head, flags | valid tokens << 8; per slot the same
+  int* meta = reinterpret_cast<int*>(state_empty + kSlots);
+  int* slot_meta = meta + kStages * 4;
+  volatile int* abort_flag = slot_meta + kSlots * 4;
   enum { kFirst = 1, kLast = 2, kPartial = 4, kPartialSlot1 = 8 };
 
   const int warp = threadIdx.x >> 5;
@@ -182,8 +189,10 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       mbar_init(smem_u32(&full_bar[s]), 2);
       mbar_init(smem_u32(&empty_bar[s]), kDecode8Warps);
     }
-    mbar_init(smem_u32(&merge_bar[0]), kDecode8Warps);
-    mbar_init(smem_u32(&merge_bar[1]), kDecode8Warps);
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(smem_u32(&state_full[s]), kDecode8Warps);
+      mbar_init(smem_u32(&state_empty[s]), kCluster ? kDecode8Warps : 1);
+    }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -208,6 +217,61 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   }
   const int Hk = p.num_kv_heads;
   const int g = p.g;
+  const float NEG_INF = -INFINITY;
+  // Sum of the consumer warps' states of one head, this lane's four dims: M, L, acc.
+  auto merge_row = [&](const float* st, int row, float& M, float& L, float4& acc) {
+    const float* src = st + row * kDecode8ORow;
+    float2 ml[kDecode8Warps];
+    M = NEG_INF;
+#pragma unroll
+    for (int w = 0; w < kDecode8Warps; ++w) {
+      ml[w] = *reinterpret_cast<const float2*>(src + w * G * kDecode8ORow + 128);
+      M = fmaxf(M, ml[w].x);
+    }
+    L = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kDecode8Warps; ++w) {
+      const float f = ml[w].x == NEG_INF ? 0.f : fast_exp2(ml[w].x - M);
+      const float4 x = *reinterpret_cast<const float4*>(src + w * G * kDecode8ORow + 4 * lane);
+      L += ml[w].y * f;
+      acc.x += x.x * f;
+      acc.y += x.y * f;
+      acc.z += x.z * f;
+      acc.w += x.w * f;
+    }
+  };
+
+  if (!kCluster && warp == kDecode8Merger) {
+    // -------------------------------------------------------------- merger
+    // Takes the states of a pair while the consumers go on with the next one,
+    // and writes its output or, if the pair is shared with other CTAs, its part.
+    for (uint32_t n = 0;; ++n) {
+      const int slot = static_cast<int>(n % kSlots);
+      if (!mbar_wait_bounded(smem_u32(&state_full[slot]), (n / kSlots) & 1u)) {
+        *abort_flag = 1;
+        return;
+      }
+      const int b = slot_meta[slot * 4], h = slot_meta[slot * 4 + 1], flags = slot_meta[slot * 4 + 2];
+      if (b < 0) return;
+#pragma unroll 2
+      for (int row = 0; row < g; ++row) {
+        float M, L;
+        float4 acc;
+        merge_row(state + slot * S::kStateFloats, row, M, L, acc);
+        if (!(flags & kPartial)) {
+          decode8_store(p.out + b * p.out_stride_token + (h * g + row) * 128 + 4 * lane, acc,
+                        L > 0.f ? 1.f / L : 0.f);
+        } else {
+          float* dst = p.parts + ((blockIdx.x * 2 + (flags & kPartialSlot1 ? 1 : 0)) * g + row) * kDecode8ORow;
+          *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
+          if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&state_empty[slot]));
+    }
+  }
 
   if (warp >= kDecode8Warps) {
     // ----------------------------------------------------------- producers
@@ -422,7 +486,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   // -------------------------------------------------------------- consumers
   const int gid = lane >> 2;
   const int tig = lane & 3;
-  const float NEG_INF = -INFINITY;
   // rows without a token
   for (int b = blockIdx.x; !kCluster && b < p.batch; b += gridDim.x) {
     if (__ldg(p.context_lens + b) > 0 && p.max_blocks > 0) continue;
@@ -637,8 +700,9 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     }
     if (!(flags & kLast)) continue;
 
-    // ---- the pair's tiles in this CTA are done: merge the warps
-    if (!mbar_wait_bounded(smem_u32(&merge_bar[1]), (merges & 1u) ^ 1u)) {
+    // ---- the pair's tiles in this CTA are done: the warp's state to shared memory
+    const int slot = static_cast<int>(merges % kSlots);
+    if (!mbar_wait_bounded(smem_u32(&state_empty[slot]), ((merges / kSlots) & 1u) ^ 1u)) {
       *abort_flag = 1;
       break;
     }
@@ -653,7 +717,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         if (head < g) {
           const float m = m_run[nt][e];
           const float f = m == NEG_INF ? 0.f : fast_exp2(w_run[nt][e] - m);
-          float* dst = state + (warp * G + head) * kDecode8ORow;
+          float* dst = state + slot * S::kStateFloats + (warp * G + head) * kDecode8ORow;
 #pragma unroll
           for (int dm = 0; dm < 8; ++dm)
             *reinterpret_cast<float2*>(dst + 16 * dm + 2 * gid) =
@@ -662,49 +726,42 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         }
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&merge_bar[0]));
-    if (!mbar_wait_bounded(smem_u32(&merge_bar[0]), merges & 1u)) {
-      *abort_flag = 1;
-      break;
+    if (!kCluster && threadIdx.x == 0) {
+      slot_meta[slot * 4] = b;
+      slot_meta[slot * 4 + 1] = h;
+      slot_meta[slot * 4 + 2] = flags;
     }
-    ++merges;
-    for (int row = warp; row < g; row += kDecode8Warps) {
-      const float* src = state + row * kDecode8ORow;
-      float M = NEG_INF;
-#pragma unroll
-      for (int w = 0; w < kDecode8Warps; ++w) M = fmaxf(M, src[w * G * kDecode8ORow + 128]);
-      float L = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kDecode8Warps; ++w) {
-        const float* ws = src + w * G * kDecode8ORow;
-        const float f = ws[128] == NEG_INF ? 0.f : fast_exp2(ws[128] - M);
-        const float4 x = *reinterpret_cast<const float4*>(ws + 4 * lane);
-        L += ws[129] * f;
-        acc.x += x.x * f;
-        acc.y += x.y * f;
-        acc.z += x.z * f;
-        acc.w += x.w * f;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&state_full[slot]));
+    if constexpr (kCluster) {
+      // one pair per CTA: the warps merge it themselves
+      if (!mbar_wait_bounded(smem_u32(&state_full[slot]), (merges / kSlots) & 1u)) {
+        *abort_flag = 1;
+        break;
       }
-      if (kCluster) {
+      for (int row = warp; row < g; row += kDecode8Warps) {
+        float M, L;
+        float4 acc;
+        merge_row(state + slot * S::kStateFloats, row, M, L, acc);
         // every tile of this CTA is consumed: the ring's memory is free
         float* dst = reinterpret_cast<float*>(smem) + row * kDecode8ORow;
         *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
         if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
-      } else if (!(flags & kPartial)) {
-        decode8_store(p.out + b * p.out_stride_token + (h * g + row) * 128 + 4 * lane, acc,
-                      L > 0.f ? 1.f / L : 0.f);
-      } else {
-        float* dst = p.parts + ((blockIdx.x * 2 + (flags & kPartialSlot1 ? 1 : 0)) * g + row) * kDecode8ORow;
-        *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
-        if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&state_empty[slot]));
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&merge_bar[1]));
+    ++merges;
   }
-  if constexpr (!kCluster) return;
+  if constexpr (!kCluster) {
+    // the end marker for the merger
+    const int slot = static_cast<int>(merges % kSlots);
+    if (!mbar_wait_bounded(smem_u32(&state_empty[slot]), ((merges / kSlots) & 1u) ^ 1u)) *abort_flag = 1;
+    if (threadIdx.x == 0) slot_meta[slot * 4] = -1;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&state_full[slot]));
+    return;
+  }
 
   // ---- cluster launch: the CTAs' rows are joined through distributed shared
   // memory, in rank order, each CTA taking some of the group's heads
@@ -767,24 +824,36 @@ __global__ void __launch_bounds__(kDecode8JoinWarps * 32) decode_fp8_join_kernel
   auto piece = [&](int i) {
     return p.parts + ((static_cast<int>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * p.g + row) * kDecode8ORow;
   };
-  float M = -INFINITY;
-  for (int i = warp + kDecode8JoinWarps * lane; i < split.pieces; i += kDecode8JoinWarps * 32)
-    M = fmaxf(M, piece(i)[128]);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-  float L = 0.f;
+  // four pieces' loads at a time, then one rescaling of the sums so far
+  float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = warp; i < split.pieces; i += kDecode8JoinWarps) {
-    const float* src = piece(i);
-    const float2 ml = *reinterpret_cast<const float2*>(src + 128);
-    const float4 x = *reinterpret_cast<const float4*>(src + 4 * lane);
-    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-    L += ml.y * f;
-    acc.x += x.x * f;
-    acc.y += x.y * f;
-    acc.z += x.z * f;
-    acc.w += x.w * f;
+  for (int i = warp; i < split.pieces; i += 4 * kDecode8JoinWarps) {
+    float2 ml[4];
+    float4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i + k * kDecode8JoinWarps < split.pieces) {
+        const float* src = piece(i + k * kDecode8JoinWarps);
+        ml[k] = *reinterpret_cast<const float2*>(src + 128);
+        x[k] = *reinterpret_cast<const float4*>(src + 4 * lane);
+      }
+    }
+    const float top = fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+    const float keep = M == -INFINITY ? 0.f : fast_exp2(M - top);
+    M = top;
+    L *= keep;
+    acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - top);
+      L += ml[k].y * f;
+      acc.x += x[k].x * f;
+      acc.y += x[k].y * f;
+      acc.z += x[k].z * f;
+      acc.w += x[k].w * f;
+    }
   }
   *reinterpret_cast<float4*>(&sums[warp][4 * lane]) = acc;
   if (lane == 0) *reinterpret_cast<float2*>(&sums[warp][128]) = make_float2(M, L);
