@@ -1312,15 +1312,16 @@ int launch_rows8(void (*kernel)(nkv::Rows8Params), const nkv::Rows8Params& p, vo
                           0, static_cast<cudaStream_t>(stream), p);
 }
 
-// 8-bit map of a cache {128 values, kv heads, slots}, boxes of `rows` slots of
-// one head, 128-byte swizzle.
-int encode_cache8(CUtensorMap* map, const void* base, int num_kv_heads, int64_t slots, int rows) {
+// 8-bit map of a cache {128 values, slots, kv heads}, boxes of `rows` slots of
+// `heads` heads (head by head in shared memory), 128-byte swizzle.
+int encode_cache8(CUtensorMap* map, const void* base, int num_kv_heads, int64_t slots, int rows,
+                  int heads) {
   auto fn = encode_fn();
   if (!fn) return NKV_ERR_CUDA;
-  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(num_kv_heads),
-                              static_cast<cuuint64_t>(slots)};
-  const cuuint64_t strides[2] = {128, static_cast<cuuint64_t>(num_kv_heads) * 128};
-  const cuuint32_t box[3] = {128, 1, static_cast<cuuint32_t>(rows)};
+  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(slots),
+                              static_cast<cuuint64_t>(num_kv_heads)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(num_kv_heads) * 128, 128};
+  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(heads)};
   const cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides,
                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1331,37 +1332,59 @@ int encode_cache8(CUtensorMap* map, const void* base, int num_kv_heads, int64_t 
 // Most tiles per CTA of a cluster launch.
 constexpr int kDecode8ClusterTiles = 12;
 
+// kv heads of a tile of the split form: two where they pair up (a token's 256
+// bytes of neighbouring heads are read together) and their q rows leave room
+// for the ring.
+int decode8_tile_heads(int g, int num_kv_heads) { return g <= 8 && num_kv_heads % 2 == 0 ? 2 : 1; }
+
 // Workspace: [split records][partials], kDecode8MaxCtas CTAs.
 constexpr size_t kDecode8SplitBytes =
     (sizeof(nkv::Decode8Split) * nkv::kDecode8MaxCtas + 255) / 256 * 256;
 size_t decode8_workspace(int g) {
-  return kDecode8SplitBytes +
-         align256(sizeof(float) * nkv::kDecode8ORow * 2 * g * nkv::kDecode8MaxCtas);
+  return kDecode8SplitBytes + align256(sizeof(float) * nkv::kDecode8ORow * 2 *
+                                       (g * decode8_tile_heads(g, 2)) * nkv::kDecode8MaxCtas);
 }
 
-// Launches with clusters of p.cluster CTAs, one per (row, kv head), where so
-// many fit at once (fewer CTAs a cluster if not), else over `grid` CTAs that
-// split the tiles. *joined: no second kernel is needed.
-template <int G>
-int launch_decode8(const CUtensorMap& tk, const CUtensorMap& tv, nkv::Decode8Params p, int grid, cudaStream_t stream,
-                   bool* joined) {
-  using S = nkv::Decode8Shape<G>;
-  static_assert(S::kSmemBytes <= kSmemOptinBytes, "shared memory of the 8-bit decode");
-  static bool attr_set[kMaxDevices] = {false};
-  static int fit[kMaxDevices][nkv::kDecode8MaxCluster + 1];  // clusters at once + 1, 0: not asked
+int set_max_smem(const void* kernel, int bytes, bool* done) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices) return NKV_ERR_CUDA;
-  auto split = nkv::paged_decode_fp8_kernel<G, false>;
-  auto cluster = nkv::paged_decode_fp8_kernel<G, true>;
-  if (!attr_set[dev]) {
-    cudaError_t e =
-        cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
-    if (e != cudaSuccess) return cuda_status(e);
-    attr_set[dev] = true;
-  }
+  if (done[dev]) return NKV_OK;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_status(e);
+  done[dev] = true;
+  return NKV_OK;
+}
+
+// Where the cache's tensor maps come from.
+struct Decode8Cache {
+  const void *k, *v;
+  int64_t slots;
+};
+
+int encode_cache8_pair(const Decode8Cache& c, const nkv::Decode8Params& p, CUtensorMap* tk,
+                       CUtensorMap* tv) {
+  const int st = encode_cache8(tk, c.k, p.num_kv_heads, c.slots, p.box_rows, p.box_heads);
+  return st != NKV_OK ? st : encode_cache8(tv, c.v, p.num_kv_heads, c.slots, p.box_rows, p.box_heads);
+}
+
+// Clusters of at most max_cluster CTAs, one per (row, kv head), if so many fit
+// at once (*launched), fewer CTAs a cluster if not.
+template <int G>
+int launch_decode8_cluster(const Decode8Cache& c, nkv::Decode8Params p, int max_cluster,
+                           cudaStream_t stream, bool* launched) {
+  using S = nkv::Decode8Shape<G, 1>;
+  static_assert(S::kSmemBytes <= kSmemOptinBytes, "shared memory of the 8-bit decode");
+  static bool attr_set[kMaxDevices] = {false};
+  static int fit[kMaxDevices][nkv::kDecode8MaxCluster + 1];  // clusters at once + 1, 0: not asked
+  auto kernel = nkv::paged_decode_fp8_kernel<G, 1, true>;
+  int st = set_max_smem(reinterpret_cast<const void*>(kernel), S::kSmemBytes, attr_set);
+  if (st != NKV_OK) return st;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  p.box_rows = std::min(p.block_size, S::kTokens);
+  p.box_heads = 1;
+  p.rows = p.g;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(nkv::kDecode8Threads<true>);
   cfg.dynamicSmemBytes = S::kSmemBytes;
@@ -1372,28 +1395,82 @@ int launch_decode8(const CUtensorMap& tk, const CUtensorMap& tv, nkv::Decode8Par
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
+  cfg.numAttrs = 2;
   const int pairs = p.batch * p.num_kv_heads;
-  for (; p.cluster > 1; --p.cluster) {
+  for (p.cluster = max_cluster; p.cluster > 1; --p.cluster) {
     cfg.gridDim = dim3(pairs * p.cluster);
-    cfg.numAttrs = 2;
     attr[1].val.clusterDim.x = p.cluster;
     int& n = fit[dev][p.cluster];
     if (n == 0) {
       int clusters = 0;
-      if (cudaOccupancyMaxActiveClusters(&clusters, cluster, &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
         cudaGetLastError();
         clusters = 0;
       }
       n = clusters + 1;
     }
-    if (n - 1 >= pairs) break;
+    if (n - 1 < pairs) continue;
+    CUtensorMap tk, tv;
+    st = encode_cache8_pair(c, p, &tk, &tv);
+    if (st != NKV_OK) return st;
+    *launched = true;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, tk, tv, p));
   }
-  *joined = p.cluster > 1;
-  if (*joined) return cuda_status(cudaLaunchKernelEx(&cfg, cluster, tk, tv, p));
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(nkv::kDecode8Threads<false>);
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, split, tk, tv, p));
+  return NKV_OK;
+}
+
+// The tiles split over the SMs, and the join behind it where a pair can be split.
+template <int G, int NH>
+int launch_decode8_split(const Decode8Cache& c, nkv::Decode8Params p, int sms, cudaStream_t stream) {
+  using S = nkv::Decode8Shape<G, NH>;
+  static_assert(S::kSmemBytes <= kSmemOptinBytes, "shared memory of the 8-bit decode");
+  static bool attr_set[kMaxDevices] = {false};
+  auto kernel = nkv::paged_decode_fp8_kernel<G, NH, false>;
+  int st = set_max_smem(reinterpret_cast<const void*>(kernel), S::kSmemBytes, attr_set);
+  if (st != NKV_OK) return st;
+  p.box_rows = std::min(p.block_size, S::kTokens);
+  p.box_heads = p.box_rows == S::kTokens ? NH : 1;
+  p.rows = p.g * NH;
+  CUtensorMap tk, tv;
+  st = encode_cache8_pair(c, p, &tk, &tv);
+  if (st != NKV_OK) return st;
+  // One CTA per SM, no more than there can be tiles. A multiple of the head
+  // groups lets the CTAs of all groups walk the same tokens in step, which the
+  // memory rewards (128 ragged rows x 8 heads, one a tile: 144 CTAs 193 us, 148
+  // CTAs 202 to 212); taken where it idles at most one SM in twenty.
+  const int groups = p.num_kv_heads / NH;
+  const int even = sms / groups * groups;
+  const int64_t row_tiles = (static_cast<int64_t>(p.max_blocks) * p.block_size + S::kTokens - 1) / S::kTokens;
+  const int grid = static_cast<int>(std::min<int64_t>(
+      sms - even <= sms / 20 ? even : sms, std::max<int64_t>(1, row_tiles * p.batch * groups)));
+  st = launch_dependent(kernel, dim3(grid), dim3(nkv::kDecode8Threads<false>), S::kSmemBytes, stream,
+                        tk, tv, p);
+  if (st != NKV_OK || row_tiles <= 1 || grid == 1) return st;
+  return launch_dependent(nkv::decode_fp8_join_kernel, dim3(grid, p.rows),
+                          dim3(nkv::kDecode8JoinWarps * 32), 0, stream, p);
+}
+
+template <int G>
+int launch_decode8(const Decode8Cache& c, const nkv::Decode8Params& p, cudaStream_t stream) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int sms = std::min(sm_count(dev), nkv::kDecode8MaxCtas);
+  const int64_t row_tiles =
+      (static_cast<int64_t>(p.max_blocks) * p.block_size + nkv::kDecode8Tile - 1) / nkv::kDecode8Tile;
+  // Clusters while every CTA of one gets few tiles: a longer row is better
+  // spread over all SMs (a cluster leaves some idle), a shorter one ends
+  // before the second kernel of the split would have started.
+  const int64_t cluster = std::min<int64_t>(
+      {nkv::kDecode8MaxCluster, row_tiles, sms / (p.batch * p.num_kv_heads)});
+  if (cluster > 1 && row_tiles <= cluster * kDecode8ClusterTiles) {
+    bool launched = false;
+    const int st = launch_decode8_cluster<G>(c, p, static_cast<int>(cluster), stream, &launched);
+    if (st != NKV_OK || launched) return st;
+  }
+  if constexpr (G <= 8) {
+    if (decode8_tile_heads(p.g, p.num_kv_heads) == 2) return launch_decode8_split<G, 2>(c, p, sms, stream);
+  }
+  return launch_decode8_split<G, 1>(c, p, sms, stream);
 }
 
 }  // namespace
@@ -1522,44 +1599,17 @@ int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.out_stride_token = out_stride_token;
-  p.box_rows = std::min(block_size, nkv::kDecode8Tile);
   p.splits = static_cast<nkv::Decode8Split*>(workspace);
   p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kDecode8SplitBytes);
-  CUtensorMap tk, tv;
-  const int64_t slots = std::max<int64_t>(num_blocks, 1) * block_size;
-  int e = encode_cache8(&tk, k_cache, num_kv_heads, slots, p.box_rows);
-  if (e == NKV_OK) e = encode_cache8(&tv, v_cache, num_kv_heads, slots, p.box_rows);
-  if (e != NKV_OK) return e;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const int sms = std::min(sm_count(dev), nkv::kDecode8MaxCtas);
-  const int pairs = batch * num_kv_heads;
-  const int64_t row_tiles = (static_cast<int64_t>(max_blocks) * block_size + nkv::kDecode8Tile - 1) /
-                            nkv::kDecode8Tile;
-  // Clusters while every CTA of one gets few tiles: a longer row is better
-  // spread over all SMs (a cluster leaves some idle), a shorter one ends
-  // before the second kernel of the split would have started.
-  const int64_t cluster = std::min<int64_t>({nkv::kDecode8MaxCluster, row_tiles, sms / pairs});
-  p.cluster = cluster > 1 && row_tiles <= cluster * kDecode8ClusterTiles ? static_cast<int>(cluster) : 1;
-  // One CTA per SM, no more than there can be tiles. A multiple of the kv
-  // heads lets the CTAs of all heads walk the same tokens in step, which the
-  // memory rewards (128 ragged rows x 8 heads: 144 CTAs 193 us, 148 CTAs 202 to
-  // 212); taken where it idles at most one SM in twenty.
-  const int even = sms / num_kv_heads * num_kv_heads;
-  const int grid = static_cast<int>(std::min<int64_t>(
-      sms - even <= sms / 20 ? even : sms, std::max<int64_t>(1, row_tiles * pairs)));
+  const Decode8Cache c{k_cache, v_cache, std::max<int64_t>(num_blocks, 1) * block_size};
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  bool joined = false;
   switch (padded_group(g)) {
-    case 1: e = launch_decode8<1>(tk, tv, p, grid, cs, &joined); break;
-    case 2: e = launch_decode8<2>(tk, tv, p, grid, cs, &joined); break;
-    case 4: e = launch_decode8<4>(tk, tv, p, grid, cs, &joined); break;
-    case 8: e = launch_decode8<8>(tk, tv, p, grid, cs, &joined); break;
-    default: e = launch_decode8<16>(tk, tv, p, grid, cs, &joined); break;
+    case 1: return launch_decode8<1>(c, p, cs);
+    case 2: return launch_decode8<2>(c, p, cs);
+    case 4: return launch_decode8<4>(c, p, cs);
+    case 8: return launch_decode8<8>(c, p, cs);
+    default: return launch_decode8<16>(c, p, cs);
   }
-  if (e != NKV_OK || joined || row_tiles <= 1 || grid == 1) return e;  // no pair can be split
-  return launch_dependent(nkv::decode_fp8_join_kernel, dim3(grid, g),
-                          dim3(nkv::kDecode8JoinWarps * 32), 0, cs, p);
 }
 
 }  // extern "C"

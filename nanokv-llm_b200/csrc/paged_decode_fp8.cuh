@@ -55,7 +55,7 @@
 
 namespace nkv {
 
-constexpr int kDecode8Tile = 128;
+constexpr int kDecode8Tile = 128;  // rows of 128 values of a tile: tokens x kv heads
 constexpr int kDecode8Warps = 8;  // consumers: two groups of four, which take the tiles in turn
 constexpr int kDecode8Merger = kDecode8Warps + 2;  // after two producers, K's and V's
 template <bool kCluster>
@@ -66,17 +66,19 @@ constexpr int kDecode8ORow = 132;   // floats of one row of a partial: O[128], m
 constexpr int kDecode8JoinWarps = 8;
 constexpr int kDecode8MaxCluster = 8;
 
-template <int G>
+template <int G, int NH>
 struct Decode8Shape {
   static_assert(G == 1 || G == 2 || G == 4 || G == 8 || G == 16, "padded group width");
+  static_assert(NH == 1 || (NH == 2 && G <= 8), "kv heads of a tile");
+  static constexpr int kTokens = kDecode8Tile / NH;  // tokens of a tile
   static constexpr int kNT = G <= 8 ? 1 : 2;  // 8-head column tiles
-  static constexpr int kStages = G <= 4 ? 6 : G <= 8 ? 5 : 4;
-  static constexpr int kQBytes = (G < 4 ? 4 : G) * 256;
+  static constexpr int kStages = NH * G <= 4 ? 6 : G <= 8 ? 5 : 4;
+  static constexpr int kQBytes = (NH * G < 4 ? 4 : NH * G) * 256;
   // [K][V][q rows][K exponents][V exponents], 1024-byte aligned
   static constexpr int kStageBytes = 2 * kDecode8TileBytes + kQBytes + 1024;
   // the warps' (O, m, l) of a pair, as many pairs as fit beside the ring
   static constexpr int kStateFloats = kDecode8Warps * G * kDecode8ORow;
-  static constexpr int kSlots = G <= 2 ? 2 : 1;
+  static constexpr int kSlots = G <= 4 && !(G == 4 && NH == 1) ? 2 : 1;
   static constexpr int kBarOffset = kStages * kStageBytes + kSlots * kStateFloats * 4;
   static constexpr int kSmemBytes = kBarOffset + (2 * kStages + 2 * kSlots) * 8 + kStages * 16 + kSlots * 16 + 16 + 1024;
 };
@@ -97,16 +99,18 @@ struct Decode8Params {
   const int32_t* context_lens;
   int max_blocks;
   int block_size;
-  int box_rows;   // tokens of one TMA box: min(block_size, 128)
+  int box_rows;   // tokens of one TMA box: min(block_size, tokens of a tile)
+  int box_heads;  // kv heads of one: a tile's where its tokens lie in one page, else 1
   int batch;
   int num_kv_heads;
   int g;
+  int rows;       // q heads of a tile's kv heads
   float scale_log2;
   __nv_bfloat16* out;
   int64_t out_stride_token;
   int cluster;           // > 1: clusters of that many CTAs, one per (row, kv head), that join by themselves
   Decode8Split* splits;  // [CTAs]
-  float* parts;          // [CTAs][2][g][kDecode8ORow]: range's first pair, last pair
+  float* parts;          // [CTAs][2][rows][kDecode8ORow]: range's first pair, last pair
 };
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -147,8 +151,9 @@ __device__ __forceinline__ int decode8_length(const Decode8Params& p, int b) {
   return len;
 }
 
+template <int NH>
 __device__ __forceinline__ int decode8_tiles(int len) {
-  return (len + kDecode8Tile - 1) / kDecode8Tile;
+  return (len + kDecode8Tile / NH - 1) / (kDecode8Tile / NH);
 }
 
 __device__ __forceinline__ void decode8_store(__nv_bfloat16* dst, float4 v, float f) {
@@ -160,11 +165,12 @@ __device__ __forceinline__ void decode8_store(__nv_bfloat16* dst, float4 v, floa
 
 // kCluster: launched as clusters of p.cluster CTAs, one per (row, kv head). (A
 // kernel of its own: the join's code in the split form cost it 3 %.)
-template <int G, bool kCluster>
+template <int G, int NH, bool kCluster>
 __global__ void __launch_bounds__(kDecode8Threads<kCluster>, 1)
 paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const Decode8Params p) {
-  using S = Decode8Shape<G>;
+  using S = Decode8Shape<G, NH>;
+  constexpr int kTokens = S::kTokens;
   constexpr int kStages = S::kStages;
   constexpr int kNT = S::kNT;
   extern __shared__ uint8_t smem_raw[];
@@ -215,25 +221,29 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     if (threadIdx.x == 0) raise_error(NKV_DEVERR_LAUNCH_SHAPE);
     return;
   }
-  const int Hk = p.num_kv_heads;
+  const int groups = p.num_kv_heads / NH;  // of kv heads, one a tile
   const int g = p.g;
   const float NEG_INF = -INFINITY;
-  // Sum of the consumer warps' states of one head, this lane's four dims: M, L, acc.
+  // Sum of the consumer warps' states of one of a tile's q heads, this lane's
+  // four dims: M, L, acc. With two kv heads a tile, every other pair of warps.
   auto merge_row = [&](const float* st, int row, float& M, float& L, float4& acc) {
-    const float* src = st + row * kDecode8ORow;
-    float2 ml[kDecode8Warps];
+    constexpr int kStates = kDecode8Warps / NH;
+    const int kvh = NH == 1 ? 0 : row / g;
+    const float* src = st + (NH == 1 ? row : 2 * kvh * G + row - kvh * g) * kDecode8ORow;
+    auto of = [](int w) { return NH == 1 ? w : (w >> 1) * 4 + (w & 1); };
+    float2 ml[kStates];
     M = NEG_INF;
 #pragma unroll
-    for (int w = 0; w < kDecode8Warps; ++w) {
-      ml[w] = *reinterpret_cast<const float2*>(src + w * G * kDecode8ORow + 128);
+    for (int w = 0; w < kStates; ++w) {
+      ml[w] = *reinterpret_cast<const float2*>(src + of(w) * G * kDecode8ORow + 128);
       M = fmaxf(M, ml[w].x);
     }
     L = 0.f;
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kDecode8Warps; ++w) {
+    for (int w = 0; w < kStates; ++w) {
       const float f = ml[w].x == NEG_INF ? 0.f : fast_exp2(ml[w].x - M);
-      const float4 x = *reinterpret_cast<const float4*>(src + w * G * kDecode8ORow + 4 * lane);
+      const float4 x = *reinterpret_cast<const float4*>(src + of(w) * G * kDecode8ORow + 4 * lane);
       L += ml[w].y * f;
       acc.x += x.x * f;
       acc.y += x.y * f;
@@ -255,15 +265,15 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       const int b = slot_meta[slot * 4], h = slot_meta[slot * 4 + 1], flags = slot_meta[slot * 4 + 2];
       if (b < 0) return;
 #pragma unroll 2
-      for (int row = 0; row < g; ++row) {
+      for (int row = 0; row < p.rows; ++row) {
         float M, L;
         float4 acc;
         merge_row(state + slot * S::kStateFloats, row, M, L, acc);
         if (!(flags & kPartial)) {
-          decode8_store(p.out + b * p.out_stride_token + (h * g + row) * 128 + 4 * lane, acc,
+          decode8_store(p.out + b * p.out_stride_token + (h * p.rows + row) * 128 + 4 * lane, acc,
                         L > 0.f ? 1.f / L : 0.f);
         } else {
-          float* dst = p.parts + ((blockIdx.x * 2 + (flags & kPartialSlot1 ? 1 : 0)) * g + row) * kDecode8ORow;
+          float* dst = p.parts + ((blockIdx.x * 2 + (flags & kPartialSlot1 ? 1 : 0)) * p.rows + row) * kDecode8ORow;
           *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
           if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
         }
@@ -285,26 +295,26 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     const uint32_t value_off = for_k ? 0u : static_cast<uint32_t>(kDecode8TileBytes);
     const uint32_t exp_off = 2 * kDecode8TileBytes + S::kQBytes + (for_k ? 0u : static_cast<uint32_t>(kDecode8Tile));
     const uint64_t policy = l2_policy_evict_first();
-    const uint32_t q_bytes = for_k ? static_cast<uint32_t>(g) * 256u : 0u;
+    const uint32_t q_bytes = for_k ? static_cast<uint32_t>(p.rows) * 256u : 0u;
     const int box_shift = 31 - __clz(p.box_rows);
-    const int tile_boxes = kDecode8Tile >> box_shift;
+    const int tile_boxes = kTokens >> box_shift;
     const int page_boxes = p.block_size >> box_shift;
     // ---- this CTA's range of tiles
     int b = 0, h = 0, t = 0, len = 0, ntiles = 0;
     int64_t u = 0, left = 0, total = 0, ctas = 1, head_tiles = 0;
     if (kCluster) {
       const int pair = static_cast<int>(blockIdx.x) / csize, rank = static_cast<int>(blockIdx.x) % csize;
-      b = pair / Hk;
-      h = pair - b * Hk;
+      b = pair / groups;
+      h = pair - b * groups;
       len = decode8_length(p, b);
-      ntiles = decode8_tiles(len);
+      ntiles = decode8_tiles<NH>(len);
       t = rank * ntiles / csize;
       left = (rank + 1) * ntiles / csize - t;
     } else {
-      for (int i = lane; i < p.batch; i += 32) head_tiles += decode8_tiles(decode8_length(p, i));
+      for (int i = lane; i < p.batch; i += 32) head_tiles += decode8_tiles<NH>(decode8_length(p, i));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) head_tiles += __shfl_xor_sync(0xffffffffu, head_tiles, o);
-      total = head_tiles * Hk;
+      total = head_tiles * groups;
       ctas = min(static_cast<int64_t>(gridDim.x), total);
       if (static_cast<int64_t>(blockIdx.x) < ctas) {
         u = blockIdx.x * total / ctas;
@@ -339,7 +349,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       int64_t rest = u - h * head_tiles;
       for (int b0 = 0;; b0 += 32) {
         load_lengths(b0);
-        int64_t incl = decode8_tiles(my_len);
+        int64_t incl = decode8_tiles<NH>(my_len);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
@@ -350,7 +360,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
           const int at = __ffs(past) - 1;
           b = b0 + at;
           len = __shfl_sync(0xffffffffu, my_len, at);
-          ntiles = decode8_tiles(len);
+          ntiles = decode8_tiles<NH>(len);
           t = static_cast<int>(rest - (__shfl_sync(0xffffffffu, incl, at) - ntiles));
           break;
         }
@@ -373,7 +383,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       const int off = ((first + lane) % page_boxes) << box_shift;
       // no page: rows far outside the tensor, which TMA fills with zeros
       slot = ok ? blk * p.block_size + off : -2 * kDecode8Tile;
-      exp_src = exps + (static_cast<int64_t>(blk) * Hk + h) * p.block_size + off;
+      exp_src = exps + (static_cast<int64_t>(blk) * p.num_kv_heads + h * NH) * p.block_size + off;
       good = __ballot_sync(0xffffffffu, ok);
     };
     if (left > 0) set_window(t * tile_boxes, load_entry(b, t * tile_boxes));
@@ -397,7 +407,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       const int seg_flags = (count == ntiles ? 0 : kPartial) | (t == 0 ? kPartialSlot1 : 0);
       if (!kCluster && t == 0 && count != ntiles) {
         const int64_t last_tile = u + ntiles - 1;
-        split.pair = b * Hk + h;
+        split.pair = b * groups + h;
         split.pieces = static_cast<int>(((last_tile + 1) * ctas - 1) / total - blockIdx.x) + 1;
       }
       // the next row: its length is at hand, its table entries are requested now
@@ -413,7 +423,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
           set_window(box0 + first, load_entry(b, box0 + first));
           first = 0;
         }
-        const int valid = min(kDecode8Tile, len - (t + j) * kDecode8Tile);
+        const int valid = min(kTokens, len - (t + j) * kTokens);
         const int boxes = (valid + p.box_rows - 1) >> box_shift;
         const int at = lane - first;
         if (at >= 0 && at < boxes) {
@@ -429,23 +439,27 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
                 m[2] = seg_flags | (j == 0 ? kFirst : 0) | (j == count - 1 ? kLast : 0) | (valid << 8);
               }
               const unsigned with_exps = (good >> first) & (0xffu >> (8 - boxes));
-              mbar_arrive_expect_tx(bar, ((boxes * 128u + __popc(with_exps)) << box_shift) +
+              mbar_arrive_expect_tx(bar, (((boxes * 128u + __popc(with_exps)) * NH) << box_shift) +
                                              (j == 0 ? q_bytes : 0u));
               if (for_k && j == 0) {
                 const __nv_bfloat16* src =
-                    p.q + b * p.q_stride_token + static_cast<int64_t>(h) * g * p.q_stride_head;
+                    p.q + b * p.q_stride_token + static_cast<int64_t>(h) * p.rows * p.q_stride_head;
                 const uint32_t sq = sbase + 2 * kDecode8TileBytes;
                 if (p.q_stride_head == 128) {
                   bulk_load_row(sq, src, q_bytes, bar);
                 } else {
-                  for (int r = 0; r < g; ++r) bulk_load_row(sq + r * 256, src + r * p.q_stride_head, 256, bar);
+                  for (int r = 0; r < p.rows; ++r) bulk_load_row(sq + r * 256, src + r * p.q_stride_head, 256, bar);
                 }
               }
             }
-            tma_load_3d(sbase + value_off + (static_cast<uint32_t>(at * 128) << box_shift), tm, bar, 0, h, slot,
-                        policy);
+            for (int hh = 0; hh < NH; hh += p.box_heads)
+              tma_load_3d(sbase + value_off + static_cast<uint32_t>((hh * kTokens + (at << box_shift)) * 128), tm,
+                          bar, 0, slot, h * NH + hh, policy);
             if ((good >> lane) & 1u) {
-              bulk_load_row(sbase + exp_off + (at << box_shift), exp_src, p.box_rows, bar);
+#pragma unroll
+              for (int hh = 0; hh < NH; ++hh)
+                bulk_load_row(sbase + exp_off + hh * kTokens + (at << box_shift), exp_src + hh * p.block_size,
+                              p.box_rows, bar);
             } else {
               raise_error(NKV_DEVERR_DECODE_BLOCK);
             }
@@ -465,7 +479,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       h = next_h;
       b = next_b;
       len = next_len;
-      ntiles = decode8_tiles(len);
+      ntiles = decode8_tiles<NH>(len);
       set_window(0, next_ent);
     }
     if (lane == 0) {
@@ -490,7 +504,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   for (int b = blockIdx.x; !kCluster && b < p.batch; b += gridDim.x) {
     if (__ldg(p.context_lens + b) > 0 && p.max_blocks > 0) continue;
     uint4* dst = reinterpret_cast<uint4*>(p.out + b * p.out_stride_token);
-    for (int i = threadIdx.x; i < Hk * g * 16; i += kDecode8Warps * 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = threadIdx.x; i < groups * p.rows * 16; i += kDecode8Warps * 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
   }
 
   float o[8][kNT][4];  // O^T: dims 16 dm + 2 gid (+ 1 for [2], [3]), heads 8 nt + 2 tig (+ 1 for odd)
@@ -501,6 +515,10 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   uint32_t phase = 0;
   uint32_t merges = 0;
   uint32_t turn = warp >> 2;  // even: the tile is this group's
+  // the warp's 32 rows of a tile: tokens tok_base .. of its kvh-th kv head
+  const int row_base = (warp & 3) * 32;
+  const int kvh = NH == 1 ? 0 : (warp & 3) >> 1;
+  const int tok_base = row_base - kvh * kTokens;
   while (true) {
     if (!mbar_wait_bounded(smem_u32(&full_bar[stage]), phase)) {
       *abort_flag = 1;
@@ -529,7 +547,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         for (int kk = 0; kk < 8; ++kk) {
           raw[kk] = make_uint2(0u, 0u);
           if (head < g)
-            raw[kk] = *reinterpret_cast<const uint2*>(sp + 2 * kDecode8TileBytes + head * 256 + kk * 32 + tig * 8);
+            raw[kk] = *reinterpret_cast<const uint2*>(sp + 2 * kDecode8TileBytes + (kvh * g + head) * 256 + kk * 32 +
+                                                      tig * 8);
           top = fmaxf(top, fmaxf(fmaxf(fabsf(__uint_as_float(raw[kk].x << 16)),
                                        fabsf(__uint_as_float(raw[kk].x & 0xffff0000u))),
                                  fmaxf(fabsf(__uint_as_float(raw[kk].y << 16)),
@@ -552,12 +571,11 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       }
     }
 
-    const int tok_base = (warp & 3) * 32;
     if ((turn++ & 1u) == 0u && tok_base < valid) {
       const uint32_t sK = smem_u32(sp);
       const uint32_t sV = sK + kDecode8TileBytes;
       const int mi = lane >> 3;
-      const int lrow = tok_base + (mi & 1) * 8 + (lane & 7);
+      const int lrow = row_base + (mi & 1) * 8 + (lane & 7);
       // ---- S^T = K Q^T: two 16-token tiles, 8 steps of 16 dims. All loads first
       // (each waits for none of the others), even and odd pairs of steps in
       // sums of their own.
@@ -600,9 +618,9 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int tk = tok_base + 16 * mt + 8 * r + gid;
-          ks[mt][r] = exp_byte_to_float(sexp[tk]);
-          vk[mt][r] = static_cast<float>(static_cast<int>(sexp[kDecode8Tile + tk]) - 127);
+          const int at = row_base + 16 * mt + 8 * r + gid;
+          ks[mt][r] = exp_byte_to_float(sexp[at]);
+          vk[mt][r] = static_cast<float>(static_cast<int>(sexp[kDecode8Tile + at]) - 127);
         }
       }
 #pragma unroll
@@ -739,7 +757,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         *abort_flag = 1;
         break;
       }
-      for (int row = warp; row < g; row += kDecode8Warps) {
+      for (int row = warp; row < p.rows; row += kDecode8Warps) {
         float M, L;
         float4 acc;
         merge_row(state + slot * S::kStateFloats, row, M, L, acc);
@@ -768,7 +786,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int rank = static_cast<int>(blockIdx.x) % csize;
   const int pair = static_cast<int>(blockIdx.x) / csize;
   if (merges == 0) {  // no tile fell to this CTA
-    for (int row = warp; row < g; row += kDecode8Warps) {
+    for (int row = warp; row < p.rows; row += kDecode8Warps) {
       float* dst = reinterpret_cast<float*>(smem) + row * kDecode8ORow;
       *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(0.f, 0.f, 0.f, 0.f);
       if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(NEG_INF, 0.f);
@@ -777,7 +795,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   __syncwarp();
   cluster_sync_all();
   const int row = warp * csize + rank;
-  if (row < g) {
+  if (row < p.rows) {
     float4 x[kDecode8MaxCluster];
     float2 ml[kDecode8MaxCluster];
     float M = NEG_INF;
@@ -803,7 +821,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       acc.z += x[c].z * f;
       acc.w += x[c].w * f;
     }
-    decode8_store(p.out + (pair / Hk) * p.out_stride_token + ((pair % Hk) * g + row) * 128 + 4 * lane, acc,
+    decode8_store(p.out + (pair / groups) * p.out_stride_token + ((pair % groups) * p.rows + row) * 128 + 4 * lane, acc,
                   L > 0.f ? 1.f / L : 0.f);
   }
   __syncwarp();
@@ -811,7 +829,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
 }
 
 // Joins the pieces of the pair that begins in CTA blockIdx.x's range and goes
-// on in later ones (head blockIdx.y of the group): each warp sums every eighth
+// on in later ones (row blockIdx.y of its q heads): each warp sums every eighth
 // piece, the first warp the eight sums, always in the same order.
 __global__ void __launch_bounds__(kDecode8JoinWarps * 32) decode_fp8_join_kernel(const Decode8Params p) {
   __shared__ float sums[kDecode8JoinWarps][kDecode8ORow];
@@ -822,7 +840,7 @@ __global__ void __launch_bounds__(kDecode8JoinWarps * 32) decode_fp8_join_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y;
   // piece 0 is the range's last pair of this CTA, piece i the first of CTA + i
   auto piece = [&](int i) {
-    return p.parts + ((static_cast<int>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * p.g + row) * kDecode8ORow;
+    return p.parts + ((static_cast<int>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row) * kDecode8ORow;
   };
   // four pieces' loads at a time, then one rescaling of the sums so far
   float M = -INFINITY, L = 0.f;
@@ -874,8 +892,9 @@ __global__ void __launch_bounds__(kDecode8JoinWarps * 32) decode_fp8_join_kernel
     acc.z += x.z * f;
     acc.w += x.w * f;
   }
-  const int b = split.pair / p.num_kv_heads, h = split.pair - b * p.num_kv_heads;
-  decode8_store(p.out + b * p.out_stride_token + (h * p.g + row) * 128 + 4 * lane, acc,
+  const int groups = p.num_kv_heads * p.g / p.rows;
+  const int b = split.pair / groups, h = split.pair - b * groups;
+  decode8_store(p.out + b * p.out_stride_token + (h * p.rows + row) * 128 + 4 * lane, acc,
                 L > 0.f ? 1.f / L : 0.f);
 }
 
