@@ -1567,8 +1567,9 @@ int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride
   if (st != NKV_OK) return st;
   const int g = num_q_heads / num_kv_heads;
   if (g > 16) return NKV_ERR_UNSUPPORTED;
-  if (static_cast<int64_t>(batch) * num_kv_heads > kMaxDecodePairs ||
-      static_cast<int64_t>(max_blocks) * block_size > 0x7fffffff)
+  const int64_t row_tokens = static_cast<int64_t>(max_blocks) * block_size;
+  if (static_cast<int64_t>(batch) * num_kv_heads > kMaxDecodePairs || row_tokens > 0x7fffff80 ||
+      row_tokens * batch > (int64_t{1} << 36) / num_kv_heads)  // the kernel counts tiles in 32 bits
     return NKV_ERR_UNSUPPORTED;
   if (!q || !out || !context_lens || (!block_tables && max_blocks > 0))
     return NKV_ERR_INVALID_ARGUMENT;

@@ -10,7 +10,7 @@
 //
 // Split and join. The work of a call is the 128-token tiles of every (row, kv
 // head) pair in the order (head, row, tile); CTA c of n takes the tiles
-// [c T / n, (c + 1) T / n). (Heads outermost: CTAs n / Hk apart then read the
+// [c T / n, (c + 1) T / n) (rounded: the first T mod n CTAs take one more). (Heads outermost: CTAs n / Hk apart then read the
 // same tokens of different heads at the same time, neighbours in memory.) Every CTA has the same number of tiles, whatever
 // the lengths, and which tiles depends on the lengths alone: results are the
 // same every time. A CTA finishes the pairs that lie inside its range; of a
@@ -127,6 +127,10 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -186,7 +190,9 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   int* meta = reinterpret_cast<int*>(state_empty + kSlots);
   int* slot_meta = meta + kStages * 4;
   volatile int* abort_flag = slot_meta + kSlots * 4;
-  enum { kFirst = 1, kLast = 2, kPartial = 4, kPartialSlot1 = 8 };
+  __shared__ int warp_tiles[kDecode8Merger + 1];
+  __shared__ int first_row[2];  // the range's first row; its tiles in the rows before
+  enum { kFirst = 1, kLast = 2, kPartial = 4, kPartialSlot1 = 8, kFinal = 16 };
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -211,6 +217,17 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   if (threadIdx.x == kDecode8Warps * 32) {
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
+  }
+  // Lengths and tables into L2 before the wait (a hint: what the kernel ahead
+  // may still write is written there too); a cache's stream has evicted them
+  // since the last call, and the first tile waits for two such loads in turn.
+  {
+    const int64_t lines = (p.batch * 4 + 127) / 128;
+    const int64_t all = lines + (static_cast<int64_t>(p.batch) * p.max_blocks * 4 + 127) / 128;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    for (int64_t i = static_cast<int64_t>(threadIdx.x) * gridDim.x + blockIdx.x; i < min(all, 4 * step); i += step)
+      prefetch_l2(i < lines ? reinterpret_cast<const char*>(p.context_lens) + i * 128
+                            : reinterpret_cast<const char*>(p.block_tables) + (i - lines) * 128);
   }
   __syncthreads();
   grid_dependency_wait();
@@ -252,10 +269,73 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     }
   };
 
+  // ---- the call's tiles and this CTA's range of them (the split form). Every
+  // thread sums the tiles of a few rows in turn; the one whose rows hold the
+  // range's first tile finds the row.
+  int total = 0, head_tiles = 0, ctas = 1, u = 0, left = 0;
+  if constexpr (!kCluster) {
+    const int per = (p.batch + static_cast<int>(blockDim.x) - 1) / static_cast<int>(blockDim.x);
+    const int row0 = min(static_cast<int>(threadIdx.x) * per, p.batch), row1 = min(row0 + per, p.batch);
+    int mine = 0;
+#pragma unroll 4
+    for (int i = row0; i < row1; ++i) mine += decode8_tiles<NH>(decode8_length(p, i));
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) warp_tiles[warp] = incl;
+    __syncthreads();
+    int before = incl - mine;
+#pragma unroll
+    for (int w = 0; w <= kDecode8Merger; ++w) {
+      const int x = warp_tiles[w];
+      if (w < warp) before += x;
+      head_tiles += x;
+    }
+    total = head_tiles * groups;
+    ctas = max(min(static_cast<int>(gridDim.x), total), 1);
+    const int c = static_cast<int>(blockIdx.x);
+    const int share = total / ctas, more = total - share * ctas;  // the first `more` CTAs take one more
+    if (c < ctas) {
+      u = c * share + min(c, more);
+      left = share + (c < more ? 1 : 0);
+    }
+    const int rest = left > 0 ? u % head_tiles : 0;
+    if (mine > 0 && rest >= before && rest < before + mine) {
+      int at = before, i = row0;
+      for (;; ++i) {
+        const int n = decode8_tiles<NH>(decode8_length(p, i));
+        if (rest < at + n) break;
+        at += n;
+      }
+      first_row[0] = i;
+      first_row[1] = at;
+    }
+    __syncthreads();
+  }
+
+  // A merged row of (b, h): the output or, if the pair is shared with other
+  // CTAs, this one's part.
+  auto put_row = [&](int slot, int b, int h, int flags, int row) {
+    float M, L;
+    float4 acc;
+    merge_row(state + slot * S::kStateFloats, row, M, L, acc);
+    if (!(flags & kPartial)) {
+      decode8_store(p.out + b * p.out_stride_token + (h * p.rows + row) * 128 + 4 * lane, acc,
+                    L > 0.f ? 1.f / L : 0.f);
+    } else {
+      float* dst = p.parts + ((blockIdx.x * 2 + (flags & kPartialSlot1 ? 1 : 0)) * p.rows + row) * kDecode8ORow;
+      *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
+      if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
+    }
+  };
+
   if (!kCluster && warp == kDecode8Merger) {
     // -------------------------------------------------------------- merger
-    // Takes the states of a pair while the consumers go on with the next one,
-    // and writes its output or, if the pair is shared with other CTAs, its part.
+    // Joins the states of a pair while the consumers go on with the next one;
+    // the last pair of the range they join themselves.
     for (uint32_t n = 0;; ++n) {
       const int slot = static_cast<int>(n % kSlots);
       if (!mbar_wait_bounded(smem_u32(&state_full[slot]), (n / kSlots) & 1u)) {
@@ -263,21 +343,9 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         return;
       }
       const int b = slot_meta[slot * 4], h = slot_meta[slot * 4 + 1], flags = slot_meta[slot * 4 + 2];
-      if (b < 0) return;
+      if (b < 0 || (flags & kFinal)) return;
 #pragma unroll 2
-      for (int row = 0; row < p.rows; ++row) {
-        float M, L;
-        float4 acc;
-        merge_row(state + slot * S::kStateFloats, row, M, L, acc);
-        if (!(flags & kPartial)) {
-          decode8_store(p.out + b * p.out_stride_token + (h * p.rows + row) * 128 + 4 * lane, acc,
-                        L > 0.f ? 1.f / L : 0.f);
-        } else {
-          float* dst = p.parts + ((blockIdx.x * 2 + (flags & kPartialSlot1 ? 1 : 0)) * p.rows + row) * kDecode8ORow;
-          *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
-          if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
-        }
-      }
+      for (int row = 0; row < p.rows; ++row) put_row(slot, b, h, flags, row);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&state_empty[slot]));
     }
@@ -299,9 +367,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     const int box_shift = 31 - __clz(p.box_rows);
     const int tile_boxes = kTokens >> box_shift;
     const int page_boxes = p.block_size >> box_shift;
-    // ---- this CTA's range of tiles
+    // ---- its first row, head and tile
     int b = 0, h = 0, t = 0, len = 0, ntiles = 0;
-    int64_t u = 0, left = 0, total = 0, ctas = 1, head_tiles = 0;
     if (kCluster) {
       const int pair = static_cast<int>(blockIdx.x) / csize, rank = static_cast<int>(blockIdx.x) % csize;
       b = pair / groups;
@@ -310,19 +377,15 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       ntiles = decode8_tiles<NH>(len);
       t = rank * ntiles / csize;
       left = (rank + 1) * ntiles / csize - t;
-    } else {
-      for (int i = lane; i < p.batch; i += 32) head_tiles += decode8_tiles<NH>(decode8_length(p, i));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) head_tiles += __shfl_xor_sync(0xffffffffu, head_tiles, o);
-      total = head_tiles * groups;
-      ctas = min(static_cast<int64_t>(gridDim.x), total);
-      if (static_cast<int64_t>(blockIdx.x) < ctas) {
-        u = blockIdx.x * total / ctas;
-        left = (blockIdx.x + 1) * total / ctas - u;
-      }
+    } else if (left > 0) {
+      b = first_row[0];
+      h = u / head_tiles;
+      t = u - h * head_tiles - first_row[1];
+      len = decode8_length(p, b);
+      ntiles = decode8_tiles<NH>(len);
     }
     // the lengths of 32 rows from lens0, one per lane
-    int lens0 = 0, my_len = 0;
+    int lens0 = -32, my_len = 0;
     auto load_lengths = [&](int first) {
       lens0 = first;
       my_len = first + lane < p.batch ? decode8_length(p, first + lane) : 0;
@@ -343,30 +406,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         row = lens0 + 32;
       }
     };
-    // ---- its first head, row and tile
-    if (!kCluster && left > 0) {
-      h = static_cast<int>(u / head_tiles);
-      int64_t rest = u - h * head_tiles;
-      for (int b0 = 0;; b0 += 32) {
-        load_lengths(b0);
-        int64_t incl = decode8_tiles<NH>(my_len);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, incl > rest);
-        if (past != 0u) {
-          const int at = __ffs(past) - 1;
-          b = b0 + at;
-          len = __shfl_sync(0xffffffffu, my_len, at);
-          ntiles = decode8_tiles<NH>(len);
-          t = static_cast<int>(rest - (__shfl_sync(0xffffffffu, incl, at) - ntiles));
-          break;
-        }
-        rest -= __shfl_sync(0xffffffffu, incl, 31);
-      }
-    }
     // the table entry of this lane's box, first + lane, of a row
     auto load_entry = [&](int row, int first) {
       const int page = (first + lane) / page_boxes;
@@ -403,20 +442,17 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     Decode8Split split{0, 0};
     while (left > 0 && ok) {
       // ---- tiles [t, t + count) of (b, h)
-      const int count = static_cast<int>(min(left, static_cast<int64_t>(ntiles - t)));
-      const int seg_flags = (count == ntiles ? 0 : kPartial) | (t == 0 ? kPartialSlot1 : 0);
+      const int count = min(left, ntiles - t);
+      const int seg_flags = (count == ntiles ? 0 : kPartial) | (t == 0 ? kPartialSlot1 : 0) |
+                            (count == left ? kFinal : 0);
       if (!kCluster && t == 0 && count != ntiles) {
-        const int64_t last_tile = u + ntiles - 1;
+        // the CTA that takes the pair's last tile
+        const int last = u + ntiles - 1, share = total / ctas, more = total - share * ctas;
+        const int cta = last < more * (share + 1) ? last / (share + 1) : more + (last - more * (share + 1)) / share;
         split.pair = b * groups + h;
-        split.pieces = static_cast<int>(((last_tile + 1) * ctas - 1) / total - blockIdx.x) + 1;
+        split.pieces = cta - static_cast<int>(blockIdx.x) + 1;
       }
-      // the next row: its length is at hand, its table entries are requested now
       int next_h = h, next_b = b + 1, next_len = 0, next_ent = -1;
-      if (left > count) {
-        seek(next_h, next_b);
-        next_len = __shfl_sync(0xffffffffu, my_len, next_b - lens0);
-        next_ent = load_entry(next_b, 0);
-      }
       for (int j = 0; j < count; ++j) {
         int first = (t + j) * tile_boxes - box0;  // the tile's first box within the window
         if (first >= 32) {
@@ -468,6 +504,12 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         ok = __all_sync(0xffffffffu, ok) != 0;
         if (!ok) break;
         ++issued;
+        if (j == 0 && left > count) {
+          // the next row: its length is at hand, its table entries are requested now
+          seek(next_h, next_b);
+          next_len = __shfl_sync(0xffffffffu, my_len, next_b - lens0);
+          next_ent = load_entry(next_b, 0);
+        }
         if (++stage == kStages) {
           stage = 0;
           phase ^= 1u;
@@ -751,28 +793,30 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&state_full[slot]));
-    if constexpr (kCluster) {
-      // one pair per CTA: the warps merge it themselves
+    if (kCluster || (flags & kFinal)) {
       if (!mbar_wait_bounded(smem_u32(&state_full[slot]), (merges / kSlots) & 1u)) {
         *abort_flag = 1;
         break;
       }
       for (int row = warp; row < p.rows; row += kDecode8Warps) {
-        float M, L;
-        float4 acc;
-        merge_row(state + slot * S::kStateFloats, row, M, L, acc);
-        // every tile of this CTA is consumed: the ring's memory is free
-        float* dst = reinterpret_cast<float*>(smem) + row * kDecode8ORow;
-        *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
-        if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
+        if constexpr (kCluster) {
+          float M, L;
+          float4 acc;
+          merge_row(state + slot * S::kStateFloats, row, M, L, acc);
+          // every tile of this CTA is consumed: the ring's memory is free
+          float* dst = reinterpret_cast<float*>(smem) + row * kDecode8ORow;
+          *reinterpret_cast<float4*>(dst + 4 * lane) = acc;
+          if (lane == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(M, L);
+        } else {
+          put_row(slot, b, h, flags, row);
+        }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&state_empty[slot]));
+      if (!kCluster) return;
     }
     ++merges;
   }
   if constexpr (!kCluster) {
-    // the end marker for the merger
+    // no tile fell to this CTA: the end marker for the merger
     const int slot = static_cast<int>(merges % kSlots);
     if (!mbar_wait_bounded(smem_u32(&state_empty[slot]), ((merges / kSlots) & 1u) ^ 1u)) *abort_flag = 1;
     if (threadIdx.x == 0) slot_meta[slot * 4] = -1;
@@ -842,14 +886,15 @@ __global__ void __launch_bounds__(kDecode8JoinWarps * 32) decode_fp8_join_kernel
   auto piece = [&](int i) {
     return p.parts + ((static_cast<int>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row) * kDecode8ORow;
   };
-  // four pieces' loads at a time, then one rescaling of the sums so far
+  // eight pieces' loads at a time, then one rescaling of the sums so far
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = warp; i < split.pieces; i += 4 * kDecode8JoinWarps) {
-    float2 ml[4];
-    float4 x[4];
+  for (int i = warp; i < split.pieces; i += 8 * kDecode8JoinWarps) {
+    float2 ml[8];
+    float4 x[8];
+    float top = M;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k) {
       ml[k] = make_float2(-INFINITY, 0.f);
       x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i + k * kDecode8JoinWarps < split.pieces) {
@@ -858,13 +903,14 @@ __global__ void __launch_bounds__(kDecode8JoinWarps * 32) decode_fp8_join_kernel
         x[k] = *reinterpret_cast<const float4*>(src + 4 * lane);
       }
     }
-    const float top = fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
     const float keep = M == -INFINITY ? 0.f : fast_exp2(M - top);
     M = top;
     L *= keep;
     acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k) {
       const float f = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - top);
       L += ml[k].y * f;
       acc.x += x[k].x * f;
