@@ -34,9 +34,9 @@ struct PageRegion {
 };
 
 // One page of a plan: tokens [0, ntok) of page src go to page dst; dst < 0:
-// nothing to do.
+// nothing to copy. shared: full pages that a fork shares.
 struct PageMove {
-  int32_t src, dst, ntok, pad;
+  int32_t src, dst, ntok, shared;
 };
 
 template <int N>
@@ -47,17 +47,70 @@ struct PageRegions {
 };
 
 // ---------------------------------------------------------------- copy
+// Tables and counts that follow a plan, updated by the kernel that copies its
+// pages (they touch nothing that the copies touch).
+struct PageTables {
+  const int32_t* in;       // block tables
+  int32_t* out;            // the same for a fork, may be for a compaction
+  int64_t entries;         // compaction: rows * max_blocks; fork: forks * max_blocks; 0: none
+  int max_blocks;
+  int64_t num_pages;
+  // fork: the rows' full pages are shared
+  const int32_t* src_rows; // null: compaction
+  const int32_t* dst_rows;
+  int32_t* ref_counts;
+  // compaction: where a page went
+  const int32_t* remap;
+};
+
+__device__ __forceinline__ void page_share(const PageTables& t, const PageMove* moves, int64_t e) {
+  const int i = static_cast<int>(e / t.max_blocks);
+  const int j = static_cast<int>(e - static_cast<int64_t>(i) * t.max_blocks);
+  if (j >= moves[i].shared) return;
+  const int32_t page = t.in[static_cast<int64_t>(t.src_rows[i]) * t.max_blocks + j];
+  if (page >= 0 && page < t.num_pages) atomicAdd(t.ref_counts + page, 1);
+  else raise_error(NKV_DEVERR_PAGES);
+  t.out[static_cast<int64_t>(t.dst_rows[i]) * t.max_blocks + j] = page;
+}
+
+__device__ __forceinline__ void page_remap(const PageTables& t, int64_t e) {
+  int32_t page = t.in[e];
+  if (page >= 0) {
+    const int32_t to = page < t.num_pages ? t.remap[page] : -2;
+    if (to >= 0) page = to;
+    else if (to == -2) raise_error(NKV_DEVERR_PAGES);  // a table names a free page, or none of the cache
+  }
+  t.out[e] = page;
+}
+
+// Bound by HBM: each page is read and written once. A CTA takes items of 32 KB,
+// every thread eight 16-byte loads and then their stores, so that a CTA has
+// 32 KB in flight.
 template <int N>
 __global__ void __launch_bounds__(kPageCopyThreads)
 page_copy_kernel(const __grid_constant__ PageRegions<N> rg, const PageMove* moves,
-                 const int32_t* num_moves_dev, int num_moves, int block_size) {
+                 const int32_t* num_moves_dev, int num_moves, const PageTables tables) {
+  constexpr int kVecs = kPageCopyBytes / 16 / kPageCopyThreads;
   allow_dependent_launch();
   grid_dependency_wait();
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kPageCopyThreads;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * kPageCopyThreads + threadIdx.x; e < tables.entries;
+       e += stride) {
+    if (tables.src_rows != nullptr) page_share(tables, moves, e);
+    else page_remap(tables, e);
+  }
+  if (rg.items_per_move == 0) return;
   const int n = num_moves_dev != nullptr ? min(*num_moves_dev, num_moves) : num_moves;
-  const int64_t total = n * rg.items_per_move;
-  for (int64_t item = blockIdx.x; item < total; item += gridDim.x) {
-    const int64_t mv = item / rg.items_per_move;
-    const int64_t rest = item - mv * rg.items_per_move;
+  // item (mv, rest) and the step of a whole grid, without a division per item
+  int64_t mv = blockIdx.x / rg.items_per_move;
+  int64_t rest = blockIdx.x - mv * rg.items_per_move;
+  const int64_t step_mv = gridDim.x / rg.items_per_move;
+  const int64_t step_rest = gridDim.x - step_mv * rg.items_per_move;
+  for (; mv < n; mv += step_mv, rest += step_rest) {
+    if (rest >= rg.items_per_move) {
+      rest -= rg.items_per_move;
+      if (++mv >= n) break;
+    }
     const PageMove move = moves[mv];
     if (move.dst < 0 || move.ntok <= 0) continue;
     int lo = 0, hi = rg.num - 1;
@@ -67,47 +120,84 @@ page_copy_kernel(const __grid_constant__ PageRegions<N> rg, const PageMove* move
       else hi = mid - 1;
     }
     const PageRegion& r = rg.r[lo];
-    const int64_t in_region = rest - r.first_item;
-    const int64_t lead = in_region / r.items_per_page;
-    const int64_t from = (in_region - lead * r.items_per_page) * kPageCopyBytes;
-    const int bytes = static_cast<int>(min(static_cast<int64_t>(kPageCopyBytes), r.page_bytes - from));
+    const uint32_t in_region = static_cast<uint32_t>(rest - r.first_item);
+    const uint32_t lead = in_region / static_cast<uint32_t>(r.items_per_page);
+    const int64_t from = static_cast<int64_t>(in_region - lead * r.items_per_page) * kPageCopyBytes;
     const int64_t live = move.ntok * r.token_bytes;  // bytes of each segment that are copied
+    const bool one_seg = r.seg_bytes == r.page_bytes;
+    if (one_seg && from >= live) continue;
+    int bytes = static_cast<int>(min(static_cast<int64_t>(kPageCopyBytes), r.page_bytes - from));
+    const bool whole = live >= r.seg_bytes;
     const uint8_t* src = r.base + lead * r.lead_stride + move.src * r.page_bytes + from;
     uint8_t* dst = r.base + lead * r.lead_stride + move.dst * r.page_bytes + from;
-    const bool whole = live >= r.seg_bytes;
-    for (int v = threadIdx.x; v < bytes / 16; v += kPageCopyThreads) {
-      const int64_t off = from + 16 * v;
-      int64_t keep = 16;
-      if (!whole) keep = live - off % r.seg_bytes;
+    // Whole 16-byte units of the item that are copied; a segment's last, partial
+    // unit (exponent bytes) goes byte by byte.
+    if (one_seg && !whole) bytes = static_cast<int>(min(static_cast<int64_t>(bytes), live - from));
+    const bool plain = (whole || one_seg) && bytes % 16 == 0;
+    if (plain) {
+      const int vecs = bytes / 16;
+      uint4 v[kVecs];
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int i = threadIdx.x + k * kPageCopyThreads;
+        if (i < vecs) v[k] = __ldcs(reinterpret_cast<const uint4*>(src) + i);
+      }
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int i = threadIdx.x + k * kPageCopyThreads;
+        if (i < vecs) __stcs(reinterpret_cast<uint4*>(dst) + i, v[k]);
+      }
+      continue;
+    }
+    const uint32_t seg = static_cast<uint32_t>(min(r.seg_bytes, static_cast<int64_t>(0x7fffffff)));
+    for (int i = threadIdx.x; i < (bytes + 15) / 16; i += kPageCopyThreads) {
+      const int64_t off = from + 16 * i;
+      int64_t keep = live - (one_seg ? off : off % seg);
       if (keep >= 16) {
-        reinterpret_cast<uint4*>(dst)[v] = reinterpret_cast<const uint4*>(src)[v];
+        reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
       } else {
-        for (int64_t i = 0; i < keep; ++i) dst[16 * v + i] = src[16 * v + i];
+        for (int64_t k = 0; k < keep; ++k) dst[16 * i + k] = src[16 * i + k];
       }
     }
   }
 }
 
 // ---------------------------------------------------------------- plan helpers
-// Exclusive prefix sum of one value per thread over the CTA; `sum` gets the total.
-__device__ __forceinline__ int block_exclusive_sum(int v, int* warp_sums, int& sum) {
+// Exclusive prefix sum of one value per warp over the CTA, the same for all
+// lanes of a warp; `sum` gets the total.
+__device__ __forceinline__ int warps_exclusive_sum(int v, int* warp_sums, int& sum) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int x = v;
+  __syncthreads();  // the previous round's sums are read
+  if (lane == 0) warp_sums[warp] = v;
+  __syncthreads();
+  int x = warp_sums[lane];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
-  __syncthreads();  // the previous round's sums are read
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  int before = 0, total = 0;
-  for (int w = 0; w < kPagePlanThreads / 32; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
+  sum = __shfl_sync(0xffffffffu, x, 31);
+  return __shfl_sync(0xffffffffu, x, warp) - v;
+}
+
+// Which of a warp's next 512 pages are in use: bit `lane` of mask k is page
+// base + 32 k + lane. Pages past the end count as neither (see `in`).
+constexpr int kPageMasks = 16;
+constexpr int kPagesPerRound = kPagePlanThreads * kPageMasks;
+__device__ __forceinline__ void page_masks(const int32_t* ref_counts, int64_t base, int64_t num_pages,
+                                           uint32_t (&used)[kPageMasks], uint32_t (&in)[kPageMasks]) {
+  const int lane = threadIdx.x & 31;
+  int32_t ref[kPageMasks];
+#pragma unroll
+  for (int k = 0; k < kPageMasks; ++k) {
+    const int64_t page = base + 32 * k + lane;
+    ref[k] = page < num_pages ? __ldcg(ref_counts + page) : 0;
   }
-  sum = total;
-  return before + x - v;
+#pragma unroll
+  for (int k = 0; k < kPageMasks; ++k) {
+    used[k] = __ballot_sync(0xffffffffu, ref[k] > 0);
+    in[k] = __ballot_sync(0xffffffffu, base + 32 * k + lane < num_pages);
+  }
 }
 
 // Drops one reference to page p (already known to be in range).
@@ -124,7 +214,6 @@ struct PageCopyPlanParams {
   const int32_t* dst;
   int n;
   int64_t num_pages;
-  int block_size;
   PageMove* moves;
 };
 
@@ -156,7 +245,7 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_copy_plan_kernel(const 
     bool ok = s >= 0 && s < p.num_pages && d >= 0 && d < p.num_pages;
     if (ok) ok = !bit_of(twice, d) && !bit_of(read, d);
     if (!ok && !skip) raise_error(NKV_DEVERR_PAGES);
-    p.moves[i] = PageMove{s, ok ? d : -1, p.block_size, 0};
+    p.moves[i] = PageMove{s, ok ? d : -1, 0x7fffffff, 0};  // every token
   }
 }
 
@@ -174,117 +263,135 @@ struct PageForkParams {
   int n;
   int32_t* out_pages;  // [n]: the page that holds the fork's last tokens, -1: none needed, -2: not forked
   PageMove* moves;     // [n]
-  int32_t* free_list;  // [n] scratch
 };
 
+// A fork as the planning CTA holds it in shared memory; dst = -1: not made.
+struct PageFork {
+  int32_t src, dst, len, page;
+};
+
+// Decides which forks can be made, releases the targets' old pages and hands
+// out a page to every fork with a partial one. (The full pages are shared by
+// the kernel that copies.) One CTA: the phases depend on each other, and each
+// is a round or two of loads.
 __global__ void __launch_bounds__(kPagePlanThreads) page_fork_plan_kernel(const PageForkParams p) {
-  extern __shared__ uint32_t maps[];  // rows read, written, written twice
+  extern __shared__ uint32_t maps[];  // rows read, written, written twice; then the forks
   __shared__ int warp_sums[kPagePlanThreads / 32];
   const int words = (p.num_rows + 31) / 32;
   uint32_t *read = maps, *written = maps + words, *twice = written + words;
-  allow_dependent_launch();
-  grid_dependency_wait();
+  PageFork* forks = reinterpret_cast<PageFork*>(maps + (3 * words + 3) / 4 * 4);
   for (int i = threadIdx.x; i < 3 * words; i += kPagePlanThreads) maps[i] = 0u;
   __syncthreads();
+  allow_dependent_launch();
+  grid_dependency_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // ---- which forks can be made: rows in range, the target named once and no source
   for (int i = threadIdx.x; i < p.n; i += kPagePlanThreads) {
     const int32_t s = p.src_rows[i], d = p.dst_rows[i];
+    forks[i] = PageFork{s, d, 0, 0};
     if (s < 0 || s >= p.num_rows || d < 0 || d >= p.num_rows) continue;
+    forks[i].len = p.context_lens[s];
     atomicOr(read + (s >> 5), 1u << (s & 31));
     if (atomicOr(written + (d >> 5), 1u << (d & 31)) >> (d & 31) & 1u)
       atomicOr(twice + (d >> 5), 1u << (d & 31));
   }
   __syncthreads();
   for (int i = threadIdx.x; i < p.n; i += kPagePlanThreads) {
-    const int32_t s = p.src_rows[i], d = p.dst_rows[i];
-    const bool skip = s == -1 && d == -1;  // padding
-    bool ok = s >= 0 && s < p.num_rows && d >= 0 && d < p.num_rows;
-    if (ok) ok = !bit_of(twice, d) && !bit_of(read, d);
-    int len = 0;
-    if (ok) {
-      len = p.context_lens[s];
-      ok = len >= 0 && len <= static_cast<int64_t>(p.max_blocks) * p.block_size;
-    }
+    const PageFork f = forks[i];
+    const bool skip = f.src == -1 && f.dst == -1;  // padding
+    bool ok = f.src >= 0 && f.src < p.num_rows && f.dst >= 0 && f.dst < p.num_rows;
+    if (ok) ok = !bit_of(twice, f.dst) && !bit_of(read, f.dst);
+    if (ok) ok = f.len >= 0 && f.len <= static_cast<int64_t>(p.max_blocks) * p.block_size;
     if (!ok && !skip) raise_error(NKV_DEVERR_PAGES);
-    // src: the source's length until the pages are known
-    p.moves[i] = PageMove{len, ok ? 0 : -1, len % p.block_size, 0};
-    p.out_pages[i] = ok ? -1 : -2;
+    if (!ok) forks[i].dst = -1;
   }
   __syncthreads();
-  // ---- the targets' old pages are released
-  const int64_t entries = static_cast<int64_t>(p.n) * p.max_blocks;
-  for (int64_t e = threadIdx.x; e < entries; e += kPagePlanThreads) {
-    const int i = static_cast<int>(e / p.max_blocks);
-    if (p.moves[i].dst < 0) continue;
-    int32_t* at = p.block_tables + static_cast<int64_t>(p.dst_rows[i]) * p.max_blocks + e % p.max_blocks;
-    const int32_t old = *at;
-    if (old >= 0) {
-      if (old < p.num_pages) page_release(p.ref_counts, old);
-      else raise_error(NKV_DEVERR_PAGES);
-      *at = -1;
+  // ---- the targets' old pages are released: a warp per target, its entries in
+  // rounds of 128 loads
+  for (int i = warp; i < p.n; i += kPagePlanThreads / 32) {
+    const int32_t d = forks[i].dst;
+    if (d < 0) continue;
+    int32_t* row = p.block_tables + static_cast<int64_t>(d) * p.max_blocks;
+    for (int j0 = 0; j0 < p.max_blocks; j0 += 128) {
+      int32_t old[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = j0 + 32 * k + lane;
+        old[k] = j < p.max_blocks ? row[j] : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (old[k] < 0) continue;
+        if (old[k] < p.num_pages) page_release(p.ref_counts, old[k]);
+        else raise_error(NKV_DEVERR_PAGES);
+        row[j0 + 32 * k + lane] = -1;
+      }
     }
   }
-  __syncthreads();
-  // ---- the lowest free pages, as many as forks want one
+  // ---- rank of every fork with a partial page among those, in order
   int want = 0;
   for (int base = 0; base < p.n; base += kPagePlanThreads) {
     const int i = base + threadIdx.x;
+    const bool wants = i < p.n && forks[i].dst >= 0 && forks[i].len % p.block_size != 0;
+    const unsigned mask = __ballot_sync(0xffffffffu, wants);
     int sum;
-    block_exclusive_sum(i < p.n && p.moves[i].dst >= 0 && p.moves[i].ntok > 0, warp_sums, sum);
+    const int before = want + warps_exclusive_sum(__popc(mask), warp_sums, sum);
+    if (i < p.n) forks[i].page = wants ? -3 - (before + __popc(mask & ((1u << lane) - 1u))) : -1;
     want += sum;
   }
+  __syncthreads();  // and the releases
+  // ---- the lowest free pages: rank r's page to the fork of rank r. The forks
+  // with a partial page, in order, start at `by_rank` (their indices).
+  int32_t* by_rank = reinterpret_cast<int32_t*>(forks + p.n);
+  for (int i = threadIdx.x; i < p.n; i += kPagePlanThreads)
+    if (forks[i].page <= -3) by_rank[-3 - forks[i].page] = i;
   int found = 0;
-  for (int64_t base = 0; base < p.num_pages && found < want; base += kPagePlanThreads) {
-    const int64_t page = base + threadIdx.x;
-    const bool free = page < p.num_pages && __ldcg(p.ref_counts + page) <= 0;
+  for (int64_t base = 0; base < p.num_pages && found < want; base += kPagesPerRound) {
+    uint32_t used[kPageMasks], in[kPageMasks];
+    const int64_t first = base + warp * 32 * kPageMasks;
+    page_masks(p.ref_counts, first, p.num_pages, used, in);
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < kPageMasks; ++k) mine += __popc(in[k] & ~used[k]);
     int sum;
-    const int rank = found + block_exclusive_sum(free, warp_sums, sum);
-    if (free && rank < want) p.free_list[rank] = static_cast<int32_t>(page);
+    int rank = found + warps_exclusive_sum(mine, warp_sums, sum);
+#pragma unroll
+    for (int k = 0; k < kPageMasks; ++k) {
+      const uint32_t free = in[k] & ~used[k];
+      const int r = rank + __popc(free & ((1u << lane) - 1u));
+      if ((free >> lane & 1u) && r < want) forks[by_rank[r]].page = static_cast<int32_t>(first + 32 * k + lane);
+      rank += __popc(free);
+    }
     found += sum;
   }
-  found = min(found, want);
   __syncthreads();
-  // ---- a page for every fork with a partial one, in the forks' order
-  int given = 0;
-  for (int base = 0; base < p.n; base += kPagePlanThreads) {
-    const int i = base + threadIdx.x;
-    const bool wants = i < p.n && p.moves[i].dst >= 0 && p.moves[i].ntok > 0;
-    int sum;
-    const int rank = given + block_exclusive_sum(wants, warp_sums, sum);
-    given += sum;
-    if (i >= p.n) continue;
-    const PageMove m = p.moves[i];
-    if (m.dst < 0) continue;
-    const int32_t s = p.src_rows[i], d = p.dst_rows[i];
-    if (wants) {
-      const int32_t from = p.block_tables[static_cast<int64_t>(s) * p.max_blocks + m.src / p.block_size];
-      if (rank >= found || from < 0 || from >= p.num_pages) {  // no page left, or none to copy
+  // ---- the plan
+  for (int i = threadIdx.x; i < p.n; i += kPagePlanThreads) {
+    const PageFork f = forks[i];
+    PageMove m{0, -1, 0, 0};
+    int32_t out = -2;
+    if (f.dst >= 0) {
+      const int full = f.len / p.block_size;
+      int32_t from = -1;
+      if (f.page != -1) from = p.block_tables[static_cast<int64_t>(f.src) * p.max_blocks + full];
+      const bool made = f.page == -1 || (f.page >= 0 && from >= 0 && from < p.num_pages);
+      if (!made) {  // no page left, or none to copy: the target stays empty
         raise_error(NKV_DEVERR_PAGES);
-        p.moves[i] = PageMove{0, -1, 0, 0};
-        p.out_pages[i] = -2;
-        p.context_lens[d] = 0;
-        continue;
+      } else {
+        out = f.page;
+        m.shared = full;
+        if (f.page >= 0) {
+          p.ref_counts[f.page] = 1;
+          p.block_tables[static_cast<int64_t>(f.dst) * p.max_blocks + full] = f.page;
+          m.src = from;
+          m.dst = f.page;
+          m.ntok = f.len - full * p.block_size;
+        }
       }
-      const int32_t to = p.free_list[rank];
-      p.ref_counts[to] = 1;
-      p.block_tables[static_cast<int64_t>(d) * p.max_blocks + m.src / p.block_size] = to;
-      p.out_pages[i] = to;
-      p.moves[i] = PageMove{from, to, m.ntok, 1 + m.src / p.block_size};
-    } else {
-      p.moves[i] = PageMove{0, -1, 0, 1 + m.src / p.block_size};
+      p.context_lens[f.dst] = made ? f.len : 0;
     }
-    p.context_lens[d] = m.src;
-  }
-  __syncthreads();
-  // ---- full pages are shared (pad: 1 + how many, 0 = not forked)
-  for (int64_t e = threadIdx.x; e < entries; e += kPagePlanThreads) {
-    const int i = static_cast<int>(e / p.max_blocks);
-    const int j = static_cast<int>(e % p.max_blocks);
-    if (j >= p.moves[i].pad - 1) continue;
-    const int32_t page = p.block_tables[static_cast<int64_t>(p.src_rows[i]) * p.max_blocks + j];
-    if (page >= 0 && page < p.num_pages) atomicAdd(p.ref_counts + page, 1);
-    else raise_error(NKV_DEVERR_PAGES);
-    p.block_tables[static_cast<int64_t>(p.dst_rows[i]) * p.max_blocks + j] = page;
+    p.moves[i] = m;
+    p.out_pages[i] = out;
   }
 }
 
@@ -329,13 +436,9 @@ __global__ void __launch_bounds__(256) page_free_kernel(const PageFreeParams p) 
 
 // ---------------------------------------------------------------- compact plan
 struct PageCompactParams {
-  const int32_t* block_tables;
-  int32_t* out_block_tables;  // may be block_tables
-  int64_t entries;            // rows * max_blocks
   const int32_t* ref_counts;
   int32_t* out_ref_counts;    // may be ref_counts
   int64_t num_pages;
-  int block_size;
   int32_t* out_num_live;
   PageMove* moves;
   int32_t* num_moves;
@@ -348,35 +451,52 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_compact_plan_kernel(con
   __shared__ int warp_sums[kPagePlanThreads / 32];
   allow_dependent_launch();
   grid_dependency_wait();
-  int live = 0;
-  for (int64_t base = 0; base < p.num_pages; base += kPagePlanThreads) {
-    const int64_t page = base + threadIdx.x;
-    int sum;
-    block_exclusive_sum(page < p.num_pages && p.ref_counts[page] > 0, warp_sums, sum);
-    live += sum;
-  }
-  int holes = 0, movers = 0;
-  for (int64_t base = 0; base < p.num_pages; base += kPagePlanThreads) {
-    const int64_t page = base + threadIdx.x;
-    const bool in = page < p.num_pages;
-    const bool used = in && p.ref_counts[page] > 0;
-    const bool hole = in && !used && page < live, mover = used && page >= live;
-    int hole_sum, mover_sum;
-    const int hole_at = holes + block_exclusive_sum(hole, warp_sums, hole_sum);
-    const int mover_at = movers + block_exclusive_sum(mover, warp_sums, mover_sum);
-    if (hole) p.moves[hole_at].dst = static_cast<int32_t>(page);
-    if (mover) p.moves[mover_at].src = static_cast<int32_t>(page);
-    if (in) {
-      p.remap[page] = used ? -1 : -2;
-      if (p.out_ref_counts != p.ref_counts) p.out_ref_counts[page] = p.ref_counts[page];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t used[kPageMasks], in[kPageMasks];
+  const int64_t warp_first = warp * 32 * kPageMasks;
+  // pages in use, and those of them below `bound`
+  auto count = [&](int64_t bound) {
+    int mine = 0;
+    for (int64_t base = 0; base < min(p.num_pages, bound); base += kPagesPerRound) {
+      page_masks(p.ref_counts, base + warp_first, min(p.num_pages, bound), used, in);
+#pragma unroll
+      for (int k = 0; k < kPageMasks; ++k) mine += __popc(used[k]);
     }
-    holes += hole_sum;
-    movers += mover_sum;
+    int sum;
+    warps_exclusive_sum(mine, warp_sums, sum);
+    return sum;
+  };
+  const int live = count(p.num_pages);
+  const int settled = count(live);  // already among the first `live`
+  int before_round = 0;             // pages in use in the rounds before
+  for (int64_t base = 0; base < p.num_pages; base += kPagesPerRound) {
+    const int64_t first = base + warp_first;
+    page_masks(p.ref_counts, first, p.num_pages, used, in);
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < kPageMasks; ++k) mine += __popc(used[k]);
+    int sum;
+    int before = before_round + warps_exclusive_sum(mine, warp_sums, sum);
+    before_round += sum;
+#pragma unroll
+    for (int k = 0; k < kPageMasks; ++k) {
+      const int64_t page = first + 32 * k + lane;
+      const int below = before + __popc(used[k] & ((1u << lane) - 1u));  // in use before this page
+      const bool is_used = used[k] >> lane & 1u;
+      if (page < p.num_pages) {
+        p.remap[page] = is_used ? -1 : -2;
+        if (p.out_ref_counts != p.ref_counts) p.out_ref_counts[page] = p.ref_counts[page];
+        if (!is_used && page < live) p.moves[page - below].dst = static_cast<int32_t>(page);
+        if (is_used && page >= live) p.moves[below - settled].src = static_cast<int32_t>(page);
+      }
+      before += __popc(used[k]);
+    }
   }
   __syncthreads();
+  const int movers = live - settled;
   for (int i = threadIdx.x; i < movers; i += kPagePlanThreads) {
     const int32_t from = p.moves[i].src, to = p.moves[i].dst;
-    p.moves[i].ntok = p.block_size;
+    p.moves[i].ntok = 0x7fffffff;  // every token
     p.remap[from] = to;
     p.out_ref_counts[to] = p.ref_counts[from];
     p.out_ref_counts[from] = 0;
@@ -385,24 +505,6 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_compact_plan_kernel(con
     *p.num_moves = movers;
     *p.out_num_live = live;
   }
-}
-
-__global__ void __launch_bounds__(256) page_remap_kernel(const PageCompactParams p) {
-  allow_dependent_launch();
-  grid_dependency_wait();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= p.entries) return;
-  int32_t page = p.block_tables[i];
-  if (page >= 0) {
-    if (page < p.num_pages) {
-      const int32_t to = p.remap[page];
-      if (to >= 0) page = to;
-      else if (to == -2) raise_error(NKV_DEVERR_PAGES);  // a table names a free page
-    } else {
-      raise_error(NKV_DEVERR_PAGES);
-    }
-  }
-  p.out_block_tables[i] = page;
 }
 
 }  // namespace nkv

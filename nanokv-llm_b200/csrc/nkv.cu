@@ -1619,15 +1619,16 @@ int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride
 namespace {
 
 constexpr int kMaxPageRegions = 256;
+constexpr int kPageCopyCtasPerSm = 8;
 
-// Workspace of the page calls: [moves: PageMove x n][int32 x (n + 4)][remap: int32 x num_pages].
+// Workspace of the page calls: [moves: PageMove x n][their number][remap: int32 x num_pages].
 struct PageWorkspace {
-  size_t off_list, off_remap, total;
+  size_t off_count, off_remap, total;
 };
 PageWorkspace page_workspace(int64_t n, int64_t num_pages) {
   PageWorkspace w;
-  w.off_list = align256(sizeof(nkv::PageMove) * static_cast<size_t>(n));
-  w.off_remap = w.off_list + align256(sizeof(int32_t) * static_cast<size_t>(n + 4));
+  w.off_count = align256(sizeof(nkv::PageMove) * static_cast<size_t>(n));
+  w.off_remap = w.off_count + 256;
   w.total = w.off_remap + align256(sizeof(int32_t) * static_cast<size_t>(num_pages));
   return w;
 }
@@ -1654,6 +1655,7 @@ int make_regions(const nkv_page_region* in, int num, int64_t num_pages, int bloc
     o.first_item = items;
     o.items_per_page = static_cast<int>((r.page_bytes + nkv::kPageCopyBytes - 1) / nkv::kPageCopyBytes);
     items += r.lead * o.items_per_page;
+    if (items > 0x7fffffff) return NKV_ERR_UNSUPPORTED;
   }
   out->num = num;
   out->items_per_move = items;
@@ -1663,29 +1665,29 @@ int make_regions(const nkv_page_region* in, int num, int64_t num_pages, int bloc
 template <int N>
 int launch_page_copy_n(const nkv_page_region* regions, int num, int64_t num_pages, int block_size,
                        const nkv::PageMove* moves, const int32_t* num_moves_dev, int64_t num_moves,
-                       void* stream) {
+                       const nkv::PageTables& tables, void* stream) {
   nkv::PageRegions<N> rg;
   const int st = make_regions(regions, num, num_pages, block_size, &rg);
   if (st != NKV_OK) return st;
-  const int64_t items = rg.items_per_move * num_moves;
-  if (items == 0) return NKV_OK;
+  const int64_t blocks = std::max(rg.items_per_move * num_moves,
+                                  (tables.entries + nkv::kPageCopyThreads - 1) / nkv::kPageCopyThreads);
+  if (blocks == 0) return NKV_OK;
   int dev = 0;
   cudaGetDevice(&dev);
-  const int64_t grid = std::min<int64_t>(items, static_cast<int64_t>(sm_count(dev)) * 8);
+  const int64_t grid = std::min<int64_t>(blocks, static_cast<int64_t>(sm_count(dev)) * kPageCopyCtasPerSm);
   return launch_dependent(nkv::page_copy_kernel<N>, dim3(static_cast<unsigned>(grid)),
                           dim3(nkv::kPageCopyThreads), 0, static_cast<cudaStream_t>(stream), rg,
-                          moves, num_moves_dev, static_cast<int>(num_moves), block_size);
+                          moves, num_moves_dev, static_cast<int>(num_moves), tables);
 }
 
 int launch_page_copy(const nkv_page_region* regions, int num, int64_t num_pages, int block_size,
                      const nkv::PageMove* moves, const int32_t* num_moves_dev, int64_t num_moves,
-                     void* stream) {
-  if (num == 0) return NKV_OK;
+                     const nkv::PageTables& tables, void* stream) {
   if (num <= 8)
     return launch_page_copy_n<8>(regions, num, num_pages, block_size, moves, num_moves_dev,
-                                 num_moves, stream);
+                                 num_moves, tables, stream);
   return launch_page_copy_n<kMaxPageRegions>(regions, num, num_pages, block_size, moves,
-                                             num_moves_dev, num_moves, stream);
+                                             num_moves_dev, num_moves, tables, stream);
 }
 
 // Regions are checked before anything is launched.
@@ -1698,7 +1700,10 @@ int check_regions(const nkv_page_region* regions, int32_t num, int64_t num_pages
 
 // Dynamic shared memory for three bit maps over `count` rows or pages.
 constexpr size_t kMaxPlanSmem = 200 * 1024;
-size_t plan_smem(int64_t count) { return 3 * sizeof(uint32_t) * static_cast<size_t>((count + 31) / 32); }
+constexpr int kMaxForks = 4096;  // of one call (they are held in shared memory)
+size_t plan_smem(int64_t count) {
+  return (3 * sizeof(uint32_t) * static_cast<size_t>((count + 31) / 32) + 15) / 16 * 16;
+}
 
 template <typename Params>
 int launch_plan(void (*kernel)(Params), const Params& p, size_t smem, bool* attr_set, void* stream) {
@@ -1743,12 +1748,12 @@ int nkv_copy_pages(const nkv_page_region* regions, int32_t num_regions, int64_t 
   p.dst = dst;
   p.n = n;
   p.num_pages = num_pages;
-  p.block_size = 0x7fffffff;  // every token
   p.moves = static_cast<nkv::PageMove*>(workspace);
   static bool attr_set[kMaxDevices] = {false};
   const int e = launch_plan(nkv::page_copy_plan_kernel, p, plan_smem(num_pages), attr_set, stream);
   if (e != NKV_OK) return e;
-  return launch_page_copy(regions, num_regions, num_pages, 0, p.moves, nullptr, n, stream);
+  return launch_page_copy(regions, num_regions, num_pages, 0, p.moves, nullptr, n,
+                          nkv::PageTables{}, stream);
 }
 
 int nkv_fork_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
@@ -1763,7 +1768,9 @@ int nkv_fork_pages(const nkv_page_region* regions, int32_t num_regions, int64_t 
   if (n == 0) return NKV_OK;
   if (!block_tables || !context_lens || !ref_counts || !src_rows || !dst_rows || !out_pages)
     return NKV_ERR_INVALID_ARGUMENT;
-  if (plan_smem(num_rows) > kMaxPlanSmem) return NKV_ERR_UNSUPPORTED;
+  // rows' bit maps and the forks, by index and by rank
+  const size_t smem = plan_smem(num_rows) + (sizeof(nkv::PageFork) + sizeof(int32_t)) * static_cast<size_t>(n);
+  if (n > kMaxForks || smem > kMaxPlanSmem) return NKV_ERR_UNSUPPORTED;
   const PageWorkspace w = page_workspace(n, 0);
   if (!workspace || workspace_bytes < w.total) return NKV_ERR_WORKSPACE;
   if (!aligned16(workspace)) return NKV_ERR_ALIGNMENT;
@@ -1780,11 +1787,18 @@ int nkv_fork_pages(const nkv_page_region* regions, int32_t num_regions, int64_t 
   p.n = n;
   p.out_pages = out_pages;
   p.moves = static_cast<nkv::PageMove*>(workspace);
-  p.free_list = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + w.off_list);
   static bool attr_set[kMaxDevices] = {false};
-  const int e = launch_plan(nkv::page_fork_plan_kernel, p, plan_smem(num_rows), attr_set, stream);
+  const int e = launch_plan(nkv::page_fork_plan_kernel, p, smem, attr_set, stream);
   if (e != NKV_OK) return e;
-  return launch_page_copy(regions, num_regions, num_pages, block_size, p.moves, nullptr, n, stream);
+  nkv::PageTables t{};
+  t.in = t.out = block_tables;
+  t.entries = static_cast<int64_t>(n) * max_blocks;
+  t.max_blocks = max_blocks;
+  t.num_pages = num_pages;
+  t.src_rows = src_rows;
+  t.dst_rows = dst_rows;
+  t.ref_counts = ref_counts;
+  return launch_page_copy(regions, num_regions, num_pages, block_size, p.moves, nullptr, n, t, stream);
 }
 
 int nkv_free_pages(int32_t* block_tables, int32_t max_blocks, int32_t num_rows,
@@ -1827,28 +1841,23 @@ int nkv_compact_pages(const nkv_page_region* regions, int32_t num_regions, int64
   if (!workspace || workspace_bytes < w.total) return NKV_ERR_WORKSPACE;
   if (!aligned16(workspace)) return NKV_ERR_ALIGNMENT;
   nkv::PageCompactParams p{};
-  p.block_tables = block_tables;
-  p.out_block_tables = out_block_tables;
-  p.entries = num_entries;
   p.ref_counts = ref_counts;
   p.out_ref_counts = out_ref_counts;
   p.num_pages = num_pages;
-  p.block_size = 0x7fffffff;
   p.out_num_live = out_num_live;
   p.moves = static_cast<nkv::PageMove*>(workspace);
-  p.num_moves = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + w.off_list);
+  p.num_moves = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + w.off_count);
   p.remap = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + w.off_remap);
-  int e = launch_dependent(nkv::page_compact_plan_kernel, dim3(1), dim3(nkv::kPagePlanThreads), 0,
-                           static_cast<cudaStream_t>(stream), p);
+  const int e = launch_dependent(nkv::page_compact_plan_kernel, dim3(1), dim3(nkv::kPagePlanThreads), 0,
+                                 static_cast<cudaStream_t>(stream), p);
   if (e != NKV_OK) return e;
-  if (num_entries > 0) {
-    const int64_t blocks = (num_entries + 255) / 256;
-    if (blocks > 0x7fffffff) return NKV_ERR_UNSUPPORTED;
-    e = launch_dependent(nkv::page_remap_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
-                         static_cast<cudaStream_t>(stream), p);
-    if (e != NKV_OK) return e;
-  }
-  return launch_page_copy(regions, num_regions, num_pages, 0, p.moves, p.num_moves, most, stream);
+  nkv::PageTables t{};
+  t.in = block_tables;
+  t.out = out_block_tables;
+  t.entries = num_entries;
+  t.num_pages = num_pages;
+  t.remap = p.remap;
+  return launch_page_copy(regions, num_regions, num_pages, 0, p.moves, p.num_moves, most, t, stream);
 }
 
 }  // extern "C"

@@ -105,6 +105,7 @@ def test_page_call_refusals():
     assert lib.nkv_fork_pages(r, 1, 10, 16, None, *fork[1:]) == BAD
     assert lib.nkv_fork_pages(r, 1, 10, 16, P, 4, 1 << 30, *fork[3:]) == UNSUPPORTED
     assert lib.nkv_fork_pages(r, 1, 10, 16, *fork[:9], None, 1 << 20, None) == WORKSPACE
+    assert lib.nkv_fork_pages(r, 1, 10, 16, *fork[:7], 4097, *fork[8:]) == UNSUPPORTED
     assert lib.nkv_free_pages(P, 4, 4, P, P, 10, 16, P, 0, 0, None) == 0
     assert lib.nkv_free_pages(P, 4, 4, P, None, 10, 16, P, 1, 0, None) == BAD
     assert lib.nkv_free_pages(P, 4, 4, P, P, 10, 0, P, 1, 0, None) == BAD
