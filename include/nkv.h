@@ -427,7 +427,8 @@ int nkv_paged_decode_static_scratch(const void* q, int64_t q_stride_token, int64
 /* byte each, addressed by slots like the bf16 cache; exponent bytes:        */
 /* [num_blocks, Hk, block_size]. Supported by every call of this section:    */
 /* head_dim 128; block_size 16, 32, 64 or a multiple of 128; num_blocks *    */
-/* block_size < 2^31; 16-byte aligned caches and exponent bytes.             */
+/* block_size < 2^31; store and read-back: num_tokens * 2 * Hk < 2^31;       */
+/* 16-byte aligned caches and exponent bytes.                                */
 
 /* Quantised slot write. Row x of token i and kv head h goes to slot         */
 /* s = slot_mapping[i] (-1: skipped; other slots outside the cache are not   */

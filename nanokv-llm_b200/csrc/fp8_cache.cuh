@@ -15,8 +15,9 @@
 // exponent bytes [num_blocks, Hk, block_size], so that the bytes of one
 // (block, kv head) lie together: a decode tile of 128 tokens takes 128 bytes.
 //
-// Both kernels only move data: 8 lanes take one row (16 elements a lane), so
-// the row maximum is three shuffles.
+// Both kernels only move data: 8 lanes take one row, lane m its elements
+// [8 m, 8 m + 8) and [64 + 8 m, 64 + 8 m + 8), so that every access of a row
+// covers whole sectors and the row maximum is three shuffles.
 #pragma once
 #include <cuda_fp8.h>
 
@@ -28,6 +29,7 @@ namespace nkv {
 constexpr int kRows8Warps = 8;      // warps per CTA
 constexpr int kRows8PerLane = 4;    // rows each group of 8 lanes takes
 constexpr int kRows8PerWarp = 4 * kRows8PerLane;
+constexpr int kLoad8Tokens = 512;   // most tokens of one CTA of the read-back
 constexpr int kRow8MinExp = -117;
 constexpr int kRow8MaxExp = 119;
 
@@ -82,44 +84,67 @@ struct Rows8Params {
   const int32_t* cu_seqlens;
   int max_blocks;
   int batch;
-  int64_t num_rows;    // tokens x 2 x Hk
+  int num_tokens;
+  uint32_t num_rows;   // tokens x 2 x Hk
+  int cta_tokens;      // read-back: tokens of one CTA
 };
 
+// Row `r` of the call: token, K (0) or V (1), kv head. The rows of a token are
+// its K heads, then its V heads.
+struct Row8 {
+  int t, which, h;
+};
+__device__ __forceinline__ Row8 row8_of(uint32_t r, int num_kv_heads) {
+  const uint32_t per_token = 2u * num_kv_heads;
+  const uint32_t t = r / per_token;
+  const int rest = static_cast<int>(r - t * per_token);
+  const int which = rest >= num_kv_heads ? 1 : 0;
+  return Row8{static_cast<int>(t), which, rest - which * num_kv_heads};
+}
+
+// Rows in three steps -- where they are, all loads, the arithmetic and the
+// stores -- so that a lane has eight 16-byte loads in flight.
 __global__ void __launch_bounds__(kRows8Warps * 32) store_kvcache_fp8_kernel(const Rows8Params p) {
   allow_dependent_launch();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
-  const int m = lane & 7;     // elements [16 m, 16 m + 16) of the row
+  const int m = lane & 7;
   const int sub = lane >> 3;  // row within the warp's four
-  const int64_t base =
-      (static_cast<int64_t>(blockIdx.x) * kRows8Warps + (threadIdx.x >> 5)) * kRows8PerWarp;
-  const int per_token = 2 * p.num_kv_heads;
+  const uint32_t base = (blockIdx.x * kRows8Warps + (threadIdx.x >> 5)) * kRows8PerWarp;
   const int64_t num_slots = p.num_blocks * p.block_size;
+  int32_t slot[kRows8PerLane];
+  Row8 row[kRows8PerLane];
+  uint4 raw[kRows8PerLane][2];
 #pragma unroll
   for (int i = 0; i < kRows8PerLane; ++i) {
-    const int64_t r = base + 4 * i + sub;
-    if (r >= p.num_rows) continue;
-    const int64_t t = r / per_token;
-    const int rest = static_cast<int>(r - t * per_token);
-    const int which = rest >= p.num_kv_heads ? 1 : 0;
-    const int h = rest - which * p.num_kv_heads;
-    const int32_t slot = __ldg(p.slot_mapping + t);
-    if (slot == -1) continue;
-    if (slot < 0 || slot >= num_slots) {
+    const uint32_t r = base + 4 * i + sub;
+    row[i] = row8_of(min(r, p.num_rows - 1), p.num_kv_heads);
+    slot[i] = r < p.num_rows ? ldg_nc_s32(p.slot_mapping + row[i].t) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kRows8PerLane; ++i) {
+    // rows that are not written are read all the same: no branch before the loads
+    const uint4* src = reinterpret_cast<const uint4*>(
+        p.src[row[i].which] + row[i].t * p.src_stride[row[i].which] + row[i].h * 128 + 8 * m);
+    raw[i][0] = ldg_nc_v4(src);
+    raw[i][1] = ldg_nc_v4(src + 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kRows8PerLane; ++i) {
+    if (slot[i] == -1) continue;
+    if (slot[i] < 0 || slot[i] >= num_slots) {
       if (m == 0) raise_error(NKV_DEVERR_STORE_SLOT);
       continue;
     }
-    const uint4* src = reinterpret_cast<const uint4*>(p.src[which] + t * p.src_stride[which] +
-                                                      static_cast<int64_t>(h) * 128 + 16 * m);
     float x[16];
     {
       float half[8];
-      bf8_to_f8(__ldg(src), half);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = half[j];
-      bf8_to_f8(__ldg(src + 1), half);
+      for (int s = 0; s < 2; ++s) {
+        bf8_to_f8(raw[i][s], half);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[8 + j] = half[j];
+        for (int j = 0; j < 8; ++j) x[8 * s + j] = half[j];
+      }
     }
     float a = 0.f;
 #pragma unroll
@@ -137,33 +162,28 @@ __global__ void __launch_bounds__(kRows8Warps * 32) store_kvcache_fp8_kernel(con
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       q[j] = e4m3x4(x[4 * j] * inv, x[4 * j + 1] * inv, x[4 * j + 2] * inv, x[4 * j + 3] * inv);
-    *reinterpret_cast<uint4*>(p.cache[which] + (static_cast<int64_t>(slot) * p.num_kv_heads + h) * 128 +
-                              16 * m) = make_uint4(q[0], q[1], q[2], q[3]);
+    uint2* dst = reinterpret_cast<uint2*>(
+        p.cache[row[i].which] + (static_cast<int64_t>(slot[i]) * p.num_kv_heads + row[i].h) * 128 + 8 * m);
+    dst[0] = make_uint2(q[0], q[1]);
+    dst[8] = make_uint2(q[2], q[3]);
     if (m == 0) {
-      const int64_t blk = slot / p.block_size;
-      p.exps[which][(blk * p.num_kv_heads + h) * p.block_size + (slot - blk * p.block_size)] =
-          static_cast<uint8_t>(k + 127);
+      const int blk = slot[i] / p.block_size;
+      p.exps[row[i].which][(static_cast<int64_t>(blk) * p.num_kv_heads + row[i].h) * p.block_size +
+                           (slot[i] - blk * p.block_size)] = static_cast<uint8_t>(k + 127);
     }
   }
 }
 
+// A CTA finds its tokens' slots first (a search, then a table entry: four or
+// five loads in turn, once for the CTA), then streams their rows.
 __global__ void __launch_bounds__(kRows8Warps * 32) load_kvcache_fp8_kernel(const Rows8Params p) {
+  __shared__ int32_t slots[kLoad8Tokens];  // -1: left as it is, -2: no page, reads as zeros
   allow_dependent_launch();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int m = lane & 7;
-  const int sub = lane >> 3;
-  const int64_t base =
-      (static_cast<int64_t>(blockIdx.x) * kRows8Warps + (threadIdx.x >> 5)) * kRows8PerWarp;
-  const int per_token = 2 * p.num_kv_heads;
-#pragma unroll
-  for (int i = 0; i < kRows8PerLane; ++i) {
-    const int64_t r = base + 4 * i + sub;
-    if (r >= p.num_rows) continue;
-    const int64_t t = r / per_token;
-    const int rest = static_cast<int>(r - t * per_token);
-    const int which = rest >= p.num_kv_heads ? 1 : 0;
-    const int h = rest - which * p.num_kv_heads;
+  const int t0 = blockIdx.x * p.cta_tokens;
+  const int tokens = min(p.cta_tokens, p.num_tokens - t0);
+  for (int i = threadIdx.x; i < tokens; i += kRows8Warps * 32) {
+    const int t = t0 + i;
     // the sequence of packed row t: the last b with cu_seqlens[b] <= t
     int lo = 0, hi = p.batch;
     while (lo < hi) {
@@ -171,41 +191,74 @@ __global__ void __launch_bounds__(kRows8Warps * 32) load_kvcache_fp8_kernel(cons
       if (__ldg(p.cu_seqlens + mid) <= t) lo = mid;
       else hi = mid - 1;
     }
-    if (lo >= p.batch) continue;  // behind the last sequence: left as it is
-    const int64_t pos = t - __ldg(p.cu_seqlens + lo);
-    if (pos < 0) continue;  // before the first sequence
-    const int64_t bi = pos / p.block_size;
-    if (bi >= p.max_blocks) {
-      if (m == 0) raise_error(NKV_DEVERR_PREFILL_RANGE);
-      continue;
-    }
-    const int32_t blk = __ldg(p.block_tables + static_cast<int64_t>(lo) * p.max_blocks + bi);
-    uint4 lo4 = make_uint4(0u, 0u, 0u, 0u), hi4 = lo4;
-    if (blk < 0 || blk >= p.num_blocks) {
-      if (m == 0) raise_error(NKV_DEVERR_DECODE_BLOCK);  // the row reads as zeros
-    } else {
-      const int off = static_cast<int>(pos - bi * p.block_size);
-      const int64_t row = (static_cast<int64_t>(blk) * p.block_size + off) * p.num_kv_heads + h;
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p.cache[which] + row * 128 + 16 * m));
-      const float s = exp_byte_to_float(__ldg(
-          p.exps[which] + (static_cast<int64_t>(blk) * p.num_kv_heads + h) * p.block_size + off));
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-      uint32_t o[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t a = e4m3x2_to_f16x2(w[j]), b = e4m3x2_hi_to_f16x2(w[j]);
-        const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a));
-        const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
-        o[2 * j] = pack_bf16x2(fa.x * s, fa.y * s);
-        o[2 * j + 1] = pack_bf16x2(fb.x * s, fb.y * s);
+    // before the first sequence or behind the last one: left as it is
+    const int pos = lo < p.batch ? t - __ldg(p.cu_seqlens + lo) : -1;
+    int slot = -1;
+    if (pos >= 0) {
+      const int bi = pos / p.block_size;
+      if (bi >= p.max_blocks) {
+        raise_error(NKV_DEVERR_PREFILL_RANGE);
+      } else {
+        const int32_t blk = __ldg(p.block_tables + static_cast<int64_t>(lo) * p.max_blocks + bi);
+        if (blk >= 0 && blk < p.num_blocks) {
+          slot = blk * p.block_size + pos - bi * p.block_size;
+        } else {
+          raise_error(NKV_DEVERR_DECODE_BLOCK);
+          slot = -2;
+        }
       }
-      lo4 = make_uint4(o[0], o[1], o[2], o[3]);
-      hi4 = make_uint4(o[4], o[5], o[6], o[7]);
     }
-    uint4* dst = reinterpret_cast<uint4*>(p.dst[which] + t * p.dst_stride[which] +
-                                          static_cast<int64_t>(h) * 128 + 16 * m);
-    dst[0] = lo4;
-    dst[1] = hi4;
+    slots[i] = slot;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const int m = lane & 7;
+  const int sub = lane >> 3;
+  const uint32_t rows = static_cast<uint32_t>(tokens) * 2u * p.num_kv_heads;
+  for (uint32_t r0 = (threadIdx.x >> 5) * kRows8PerWarp; r0 < rows; r0 += kRows8Warps * kRows8PerWarp) {
+    Row8 row[kRows8PerLane];
+    int slot[kRows8PerLane];
+    uint2 raw[kRows8PerLane][2];
+    uint32_t byte[kRows8PerLane];
+#pragma unroll
+    for (int i = 0; i < kRows8PerLane; ++i) {
+      const uint32_t r = r0 + 4 * i + sub;
+      row[i] = row8_of(min(r, rows - 1), p.num_kv_heads);
+      slot[i] = r < rows ? slots[row[i].t] : -1;
+      raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
+      byte[i] = 0u;
+      if (slot[i] >= 0) {
+        const uint2* src = reinterpret_cast<const uint2*>(
+            p.cache[row[i].which] + (static_cast<int64_t>(slot[i]) * p.num_kv_heads + row[i].h) * 128 + 8 * m);
+        const int blk = slot[i] / p.block_size;
+        raw[i][0] = __ldg(src);
+        raw[i][1] = __ldg(src + 8);
+        byte[i] = __ldg(p.exps[row[i].which] +
+                        (static_cast<int64_t>(blk) * p.num_kv_heads + row[i].h) * p.block_size +
+                        (slot[i] - blk * p.block_size));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows8PerLane; ++i) {
+      if (slot[i] == -1) continue;
+      const float s = exp_byte_to_float(byte[i]);
+      uint4* dst = reinterpret_cast<uint4*>(p.dst[row[i].which] +
+                                            (t0 + row[i].t) * p.dst_stride[row[i].which] + row[i].h * 128 + 8 * m);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t w[2] = {raw[i][half].x, raw[i][half].y};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t a = e4m3x2_to_f16x2(w[j]), b = e4m3x2_hi_to_f16x2(w[j]);
+          const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a));
+          const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
+          o[2 * j] = pack_bf16x2(fa.x * s, fa.y * s);
+          o[2 * j + 1] = pack_bf16x2(fb.x * s, fb.y * s);
+        }
+        dst[8 * half] = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
   }
 }
 
