@@ -27,8 +27,7 @@
 namespace nkv {
 
 constexpr int kRows8Warps = 8;      // warps per CTA
-constexpr int kRows8PerLane = 4;    // rows each group of 8 lanes takes
-constexpr int kRows8PerWarp = 4 * kRows8PerLane;
+constexpr int kRows8PerLane = 2;    // rows a group of 8 lanes takes at a time
 constexpr int kLoad8Tokens = 512;   // most tokens of one CTA of the read-back
 constexpr int kRow8MinExp = -117;
 constexpr int kRow8MaxExp = 119;
@@ -38,14 +37,44 @@ __device__ __forceinline__ float exp_byte_to_float(uint32_t byte) {
   return __uint_as_float(byte << 23);
 }
 
-// k of the row maximum a (finite, >= 0): a = 1.f * 2^e needs k = e - 8 while
-// 1.f <= 1.75 (448 = 1.75 * 2^8), else e - 7. bf16 subnormals have a zero
-// exponent field and land below the lower bound either way.
-__device__ __forceinline__ int row8_exponent(float a) {
-  const uint32_t bits = __float_as_uint(a);
-  const int e = static_cast<int>(bits >> 23) - 127;
-  const int k = e - 8 + ((bits & 0x007fffffu) > 0x00600000u ? 1 : 0);
+// k of a row from its maximum's bf16 bits (finite): a = 1.f * 2^e needs
+// k = e - 8 while 1.f <= 1.75 (448 = 1.75 * 2^8), else e - 7. Zero and subnormal
+// maxima have a zero exponent field and land below the lower bound.
+__device__ __forceinline__ int row8_exponent(uint32_t bits) {
+  const int k = static_cast<int>(bits >> 7) - 127 - 8 + ((bits & 0x7fu) > 0x60u ? 1 : 0);
   return min(max(k, kRow8MinExp), kRow8MaxExp);
+}
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// bf16 bits of the largest finite magnitude among the 16 elements that each of
+// a row's 8 lanes holds (magnitudes of bf16 numbers order as their bits do).
+__device__ __forceinline__ uint32_t row8_top(const uint4 (&raw)[2], unsigned mask) {
+  const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+  auto reduce = [&](uint32_t v) {
+    v = max_u16x2(v, __shfl_xor_sync(mask, v, 1));
+    v = max_u16x2(v, __shfl_xor_sync(mask, v, 2));
+    v = max_u16x2(v, __shfl_xor_sync(mask, v, 4));
+    return max(v & 0xffffu, v >> 16);
+  };
+  uint32_t v = 0u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v = max_u16x2(v, w[j] & 0x7fff7fffu);
+  uint32_t top = reduce(v);
+  if (top >= 0x7f80u) {  // infinities and NaN do not set the scale
+    v = 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t a = w[j] & 0x7fff7fffu;
+      v = max_u16x2(v, ((a & 0xffffu) < 0x7f80u ? a & 0xffffu : 0u) | (a < 0x7f800000u ? a & 0xffff0000u : 0u));
+    }
+    top = reduce(v);
+  }
+  return top;
 }
 
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
@@ -85,99 +114,95 @@ struct Rows8Params {
   int max_blocks;
   int batch;
   int num_tokens;
-  uint32_t num_rows;   // tokens x 2 x Hk
-  int cta_tokens;      // read-back: tokens of one CTA
+  int cta_tokens;      // tokens of one CTA
 };
 
-// Row `r` of the call: token, K (0) or V (1), kv head. The rows of a token are
-// its K heads, then its V heads.
-struct Row8 {
-  int t, which, h;
+// What a group of 8 lanes does in a CTA: a token's rows are its K heads, then
+// its V heads; the CTA's 32 groups take `width` rows of `tokens` tokens at a
+// time, a group always the same row of its tokens, so that only the token
+// changes from one access to the next.
+struct Rows8Group {
+  int which, h, first, tokens;  // K (0) or V (1), kv head, first token, tokens of a pass
 };
-__device__ __forceinline__ Row8 row8_of(uint32_t r, int num_kv_heads) {
-  const uint32_t per_token = 2u * num_kv_heads;
-  const uint32_t t = r / per_token;
-  const int rest = static_cast<int>(r - t * per_token);
-  const int which = rest >= num_kv_heads ? 1 : 0;
-  return Row8{static_cast<int>(t), which, rest - which * num_kv_heads};
+__device__ __forceinline__ bool rows8_group(int row0, int num_kv_heads, Rows8Group& g) {
+  constexpr int kGroups = kRows8Warps * 4;
+  const int width = min(2 * num_kv_heads - row0, kGroups);
+  const int group = threadIdx.x >> 3;
+  g.tokens = kGroups / width;
+  g.first = group / width;
+  const int row = row0 + group - g.first * width;
+  g.which = row >= num_kv_heads ? 1 : 0;
+  g.h = row - g.which * num_kv_heads;
+  return g.first < g.tokens;
 }
 
-// Rows in three steps -- where they are, all loads, the arithmetic and the
-// stores -- so that a lane has eight 16-byte loads in flight.
+// Both kernels: a pass takes kRows8PerLane tokens a group, their loads first,
+// then the arithmetic and the stores.
 __global__ void __launch_bounds__(kRows8Warps * 32) store_kvcache_fp8_kernel(const Rows8Params p) {
   allow_dependent_launch();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int m = lane & 7;
-  const int sub = lane >> 3;  // row within the warp's four
-  const uint32_t base = (blockIdx.x * kRows8Warps + (threadIdx.x >> 5)) * kRows8PerWarp;
+  const int m = threadIdx.x & 7;
+  const unsigned mask = 0xffu << (threadIdx.x & 24);  // this row's 8 lanes, all on the same path
+  const int t0 = blockIdx.x * p.cta_tokens;
+  const int tokens = min(p.cta_tokens, p.num_tokens - t0);
   const int64_t num_slots = p.num_blocks * p.block_size;
-  int32_t slot[kRows8PerLane];
-  Row8 row[kRows8PerLane];
-  uint4 raw[kRows8PerLane][2];
+  for (int row0 = 0; row0 < 2 * p.num_kv_heads; row0 += kRows8Warps * 4) {
+    Rows8Group g;
+    if (!rows8_group(row0, p.num_kv_heads, g)) continue;
+    const int64_t src_stride = p.src_stride[g.which];
+    const __nv_bfloat16* src = p.src[g.which] + t0 * src_stride + g.h * 128 + 8 * m;
+    uint8_t* values = p.cache[g.which] + g.h * 128 + 8 * m;
+    uint8_t* exps = p.exps[g.which] + static_cast<int64_t>(g.h) * p.block_size;
+    for (int t = g.first; t < tokens; t += g.tokens * kRows8PerLane) {
+      int32_t slot[kRows8PerLane];
+      uint4 raw[kRows8PerLane][2];
 #pragma unroll
-  for (int i = 0; i < kRows8PerLane; ++i) {
-    const uint32_t r = base + 4 * i + sub;
-    row[i] = row8_of(min(r, p.num_rows - 1), p.num_kv_heads);
-    slot[i] = r < p.num_rows ? ldg_nc_s32(p.slot_mapping + row[i].t) : -1;
-  }
-#pragma unroll
-  for (int i = 0; i < kRows8PerLane; ++i) {
-    // rows that are not written are read all the same: no branch before the loads
-    const uint4* src = reinterpret_cast<const uint4*>(
-        p.src[row[i].which] + row[i].t * p.src_stride[row[i].which] + row[i].h * 128 + 8 * m);
-    raw[i][0] = ldg_nc_v4(src);
-    raw[i][1] = ldg_nc_v4(src + 8);
-  }
-#pragma unroll
-  for (int i = 0; i < kRows8PerLane; ++i) {
-    if (slot[i] == -1) continue;
-    if (slot[i] < 0 || slot[i] >= num_slots) {
-      if (m == 0) raise_error(NKV_DEVERR_STORE_SLOT);
-      continue;
-    }
-    float x[16];
-    {
-      float half[8];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bf8_to_f8(raw[i][s], half);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[8 * s + j] = half[j];
+      for (int i = 0; i < kRows8PerLane; ++i) {
+        const int tt = t + i * g.tokens;
+        slot[i] = -1;
+        if (tt >= tokens) continue;
+        slot[i] = ldg_nc_s32(p.slot_mapping + t0 + tt);
+        // read whatever the slot is: no wait before the loads
+        const uint4* at = reinterpret_cast<const uint4*>(src + tt * src_stride);
+        raw[i][0] = ldg_nc_v4(at);
+        raw[i][1] = ldg_nc_v4(at + 8);
       }
-    }
-    float a = 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float v = fabsf(x[j]);
-      if (v < INFINITY) a = fmaxf(a, v);  // infinities and NaN do not set the scale
-    }
-    const unsigned mask = 0xffu << (8 * sub);  // this row's 8 lanes, all on the same path
-    a = fmaxf(a, __shfl_xor_sync(mask, a, 1));
-    a = fmaxf(a, __shfl_xor_sync(mask, a, 2));
-    a = fmaxf(a, __shfl_xor_sync(mask, a, 4));
-    const int k = row8_exponent(a);
-    const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-    uint32_t q[4];
+      for (int i = 0; i < kRows8PerLane; ++i) {
+        if (slot[i] == -1) continue;
+        if (slot[i] < 0 || slot[i] >= num_slots) {
+          if (m == 0) raise_error(NKV_DEVERR_STORE_SLOT);
+          continue;
+        }
+        float x[2][8];
+        bf8_to_f8(raw[i][0], x[0]);
+        bf8_to_f8(raw[i][1], x[1]);
+        const int k = row8_exponent(row8_top(raw[i], mask));
+        const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+        uint2 q[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      q[j] = e4m3x4(x[4 * j] * inv, x[4 * j + 1] * inv, x[4 * j + 2] * inv, x[4 * j + 3] * inv);
-    uint2* dst = reinterpret_cast<uint2*>(
-        p.cache[row[i].which] + (static_cast<int64_t>(slot[i]) * p.num_kv_heads + row[i].h) * 128 + 8 * m);
-    dst[0] = make_uint2(q[0], q[1]);
-    dst[8] = make_uint2(q[2], q[3]);
-    if (m == 0) {
-      const int blk = slot[i] / p.block_size;
-      p.exps[row[i].which][(static_cast<int64_t>(blk) * p.num_kv_heads + row[i].h) * p.block_size +
-                           (slot[i] - blk * p.block_size)] = static_cast<uint8_t>(k + 127);
+        for (int half = 0; half < 2; ++half) {
+          const float(&v)[8] = x[half];
+          q[half] = make_uint2(e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                               e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+        }
+        uint2* dst = reinterpret_cast<uint2*>(values + static_cast<int64_t>(slot[i]) * p.num_kv_heads * 128);
+        dst[0] = q[0];
+        dst[8] = q[1];
+        if (m == 0) {
+          const int blk = slot[i] / p.block_size;
+          exps[static_cast<int64_t>(blk) * p.num_kv_heads * p.block_size + (slot[i] - blk * p.block_size)] =
+              static_cast<uint8_t>(k + 127);
+        }
+      }
     }
   }
 }
 
-// A CTA finds its tokens' slots first (a search, then a table entry: four or
+// A CTA finds its tokens' pages first (a search, then a table entry: four or
 // five loads in turn, once for the CTA), then streams their rows.
 __global__ void __launch_bounds__(kRows8Warps * 32) load_kvcache_fp8_kernel(const Rows8Params p) {
-  __shared__ int32_t slots[kLoad8Tokens];  // -1: left as it is, -2: no page, reads as zeros
+  __shared__ int2 places[kLoad8Tokens];  // block, offset in it; block -1: left as it is, -2: reads as zeros
   allow_dependent_launch();
   grid_dependency_wait();
   const int t0 = blockIdx.x * p.cta_tokens;
@@ -193,70 +218,71 @@ __global__ void __launch_bounds__(kRows8Warps * 32) load_kvcache_fp8_kernel(cons
     }
     // before the first sequence or behind the last one: left as it is
     const int pos = lo < p.batch ? t - __ldg(p.cu_seqlens + lo) : -1;
-    int slot = -1;
+    int2 place = make_int2(-1, 0);
     if (pos >= 0) {
       const int bi = pos / p.block_size;
       if (bi >= p.max_blocks) {
         raise_error(NKV_DEVERR_PREFILL_RANGE);
       } else {
-        const int32_t blk = __ldg(p.block_tables + static_cast<int64_t>(lo) * p.max_blocks + bi);
-        if (blk >= 0 && blk < p.num_blocks) {
-          slot = blk * p.block_size + pos - bi * p.block_size;
-        } else {
+        place = make_int2(__ldg(p.block_tables + static_cast<int64_t>(lo) * p.max_blocks + bi),
+                          pos - bi * p.block_size);
+        if (place.x < 0 || place.x >= p.num_blocks) {
           raise_error(NKV_DEVERR_DECODE_BLOCK);
-          slot = -2;
+          place.x = -2;
         }
       }
     }
-    slots[i] = slot;
+    places[i] = place;
   }
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  const int m = lane & 7;
-  const int sub = lane >> 3;
-  const uint32_t rows = static_cast<uint32_t>(tokens) * 2u * p.num_kv_heads;
-  for (uint32_t r0 = (threadIdx.x >> 5) * kRows8PerWarp; r0 < rows; r0 += kRows8Warps * kRows8PerWarp) {
-    Row8 row[kRows8PerLane];
-    int slot[kRows8PerLane];
-    uint2 raw[kRows8PerLane][2];
-    uint32_t byte[kRows8PerLane];
+  const int m = threadIdx.x & 7;
+  for (int row0 = 0; row0 < 2 * p.num_kv_heads; row0 += kRows8Warps * 4) {
+    Rows8Group g;
+    if (!rows8_group(row0, p.num_kv_heads, g)) continue;
+    const int64_t dst_stride = p.dst_stride[g.which];
+    __nv_bfloat16* out = p.dst[g.which] + t0 * dst_stride + g.h * 128 + 8 * m;
+    const int64_t block_rows = static_cast<int64_t>(p.num_kv_heads) * p.block_size;
+    const uint8_t* values = p.cache[g.which] + g.h * 128 + 8 * m;
+    const uint8_t* exps = p.exps[g.which] + static_cast<int64_t>(g.h) * p.block_size;
+    for (int t = g.first; t < tokens; t += g.tokens * kRows8PerLane) {
+      int blk[kRows8PerLane];
+      uint2 raw[kRows8PerLane][2];
+      uint32_t byte[kRows8PerLane];
 #pragma unroll
-    for (int i = 0; i < kRows8PerLane; ++i) {
-      const uint32_t r = r0 + 4 * i + sub;
-      row[i] = row8_of(min(r, rows - 1), p.num_kv_heads);
-      slot[i] = r < rows ? slots[row[i].t] : -1;
-      raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
-      byte[i] = 0u;
-      if (slot[i] >= 0) {
-        const uint2* src = reinterpret_cast<const uint2*>(
-            p.cache[row[i].which] + (static_cast<int64_t>(slot[i]) * p.num_kv_heads + row[i].h) * 128 + 8 * m);
-        const int blk = slot[i] / p.block_size;
-        raw[i][0] = __ldg(src);
-        raw[i][1] = __ldg(src + 8);
-        byte[i] = __ldg(p.exps[row[i].which] +
-                        (static_cast<int64_t>(blk) * p.num_kv_heads + row[i].h) * p.block_size +
-                        (slot[i] - blk * p.block_size));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kRows8PerLane; ++i) {
-      if (slot[i] == -1) continue;
-      const float s = exp_byte_to_float(byte[i]);
-      uint4* dst = reinterpret_cast<uint4*>(p.dst[row[i].which] +
-                                            (t0 + row[i].t) * p.dst_stride[row[i].which] + row[i].h * 128 + 8 * m);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t w[2] = {raw[i][half].x, raw[i][half].y};
-        uint32_t o[4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t a = e4m3x2_to_f16x2(w[j]), b = e4m3x2_hi_to_f16x2(w[j]);
-          const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a));
-          const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
-          o[2 * j] = pack_bf16x2(fa.x * s, fa.y * s);
-          o[2 * j + 1] = pack_bf16x2(fb.x * s, fb.y * s);
+      for (int i = 0; i < kRows8PerLane; ++i) {
+        const int tt = t + i * g.tokens;
+        const int2 place = tt < tokens ? places[tt] : make_int2(-1, 0);
+        blk[i] = place.x;
+        raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
+        byte[i] = 0u;
+        if (place.x >= 0) {
+          const int64_t base = place.x * block_rows;
+          const uint2* src =
+              reinterpret_cast<const uint2*>(values + (base + place.y * p.num_kv_heads) * 128);
+          raw[i][0] = __ldg(src);
+          raw[i][1] = __ldg(src + 8);
+          byte[i] = __ldg(exps + base + place.y);
         }
-        dst[8 * half] = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+#pragma unroll
+      for (int i = 0; i < kRows8PerLane; ++i) {
+        if (blk[i] == -1) continue;
+        const float s = exp_byte_to_float(byte[i]);
+        uint4* dst = reinterpret_cast<uint4*>(out + (t + i * g.tokens) * dst_stride);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t w[2] = {raw[i][half].x, raw[i][half].y};
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t a = e4m3x2_to_f16x2(w[j]), b = e4m3x2_hi_to_f16x2(w[j]);
+            const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a));
+            const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
+            o[2 * j] = pack_bf16x2(fa.x * s, fa.y * s);
+            o[2 * j + 1] = pack_bf16x2(fb.x * s, fb.y * s);
+          }
+          dst[8 * half] = make_uint4(o[0], o[1], o[2], o[3]);
+        }
       }
     }
   }
