@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import math
 import threading
+from array import array
 
 import torch
 
@@ -467,38 +468,49 @@ def threshold_compress(ring: torch.Tensor, ring_slot_of_selected: torch.Tensor, 
 
 
 # ---------------------------------------------------------------- 8-bit cache
-def _one_device(name: str, first: torch.Tensor, *tensors: torch.Tensor | None) -> torch.device:
-    """The CUDA device all tensors are on."""
-    device = first.device
-    if device.type != "cuda":
-        raise ValueError(f"{name}: CUDA tensors required (libnkv has no CPU path)")
+# These calls are short, so their host side counts: one pass over the arguments,
+# strides and shapes read once, the raw stream of the device.
+def _one_device(name: str, *tensors: torch.Tensor | None) -> int:
+    """The index of the CUDA device all tensors are on."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"{name}: all tensors must be on one CUDA device")
-    return device
+    if index < 0:
+        raise ValueError(f"{name}: CUDA tensors required (libnkv has no CPU path)")
+    return index
 
 
-def _call(device: torch.device, name: str, *args) -> None:
+def _call(device: int, name: str, *args) -> None:
     """Entry point `name` on the device's current stream, with that device current."""
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device == torch.cuda.current_device():
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(name, status)
+            status = fn(*args, stream)
+    if status:
+        _lib.check(name, status)
 
 
-def _check_cache8(k_cache, v_cache, k_exp, v_exp) -> tuple[int, int, int, int]:
+def _check_cache8(k_cache, v_cache, k_exp, v_exp) -> torch.Size:
     """(num_blocks, block_size, Hk, D) of an 8-bit cache."""
-    num_blocks, block_size, Hk, D = k_cache.shape
-    assert v_cache.shape == k_cache.shape
-    assert k_cache.dtype == torch.float8_e4m3fn and v_cache.dtype == torch.float8_e4m3fn
-    assert k_exp.shape == (num_blocks, Hk, block_size) and v_exp.shape == k_exp.shape
-    assert k_exp.dtype == torch.uint8 and v_exp.dtype == torch.uint8
+    shape = k_cache.shape
+    num_blocks, block_size, Hk, _ = shape
+    exp_shape = k_exp.shape
+    assert v_cache.shape == shape and v_exp.shape == exp_shape
+    assert exp_shape == (num_blocks, Hk, block_size)
+    assert k_cache.dtype is _E4M3 and v_cache.dtype is _E4M3
+    assert k_exp.dtype is torch.uint8 and v_exp.dtype is torch.uint8
     assert k_cache.is_contiguous() and v_cache.is_contiguous()
     assert k_exp.is_contiguous() and v_exp.is_contiguous()
-    return num_blocks, block_size, Hk, D
+    return shape
+
+
+_E4M3 = torch.float8_e4m3fn
+_BF16 = torch.bfloat16
+_INT32 = torch.int32
 
 
 def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -515,18 +527,19 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     """
     device = _one_device("store_kvcache_fp8", key, value, k_cache, v_cache, k_exp, v_exp,
                          slot_mapping)
-    N, num_heads, head_dim = key.shape
     num_blocks, block_size, Hk, D = _check_cache8(k_cache, v_cache, k_exp, v_exp)
-    assert value.shape == key.shape and (num_heads, head_dim) == (Hk, D)
-    assert key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16
-    assert key.stride(-1) == 1 and value.stride(-1) == 1
-    assert key.stride(1) == D and value.stride(1) == D
-    assert slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous()
+    shape = key.shape
+    N = shape[0]
+    k_stride, v_stride = key.stride(), value.stride()
+    assert shape == (N, Hk, D) and value.shape == shape
+    assert key.dtype is _BF16 and value.dtype is _BF16
+    assert k_stride[1:] == (D, 1) and v_stride[1:] == (D, 1)
+    assert slot_mapping.dtype is _INT32 and slot_mapping.is_contiguous()
     assert slot_mapping.numel() == N
     if N == 0 or num_blocks == 0:
         return
-    _call(device, "nkv_store_kvcache_fp8", key.data_ptr(), key.stride(0), value.data_ptr(),
-          value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(),
+    _call(device, "nkv_store_kvcache_fp8", key.data_ptr(), k_stride[0], value.data_ptr(),
+          v_stride[0], k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(),
           v_exp.data_ptr(), num_blocks, block_size, slot_mapping.data_ptr(), N, Hk, D)
 
 
@@ -546,24 +559,25 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.
                          cu_seqlens, k_out, v_out)
     num_blocks, block_size, Hk, D = _check_cache8(k_cache, v_cache, k_exp, v_exp)
     B = cu_seqlens.numel() - 1
-    assert cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and B >= 0
-    assert block_tables.dtype == torch.int32 and block_tables.dim() == 2
-    assert block_tables.size(0) >= B and num_tokens >= 0
+    assert cu_seqlens.dtype is _INT32 and cu_seqlens.is_contiguous() and B >= 0
+    rows, max_blocks = block_tables.shape
+    assert block_tables.dtype is _INT32 and rows >= B and num_tokens >= 0
     if not block_tables.is_contiguous():
         block_tables = block_tables.contiguous()
     if k_out is None:
-        k_out = torch.empty(num_tokens, Hk, D, dtype=torch.bfloat16, device=device)
+        k_out = k_cache.new_empty((num_tokens, Hk, D), dtype=_BF16)
     if v_out is None:
-        v_out = torch.empty(num_tokens, Hk, D, dtype=torch.bfloat16, device=device)
-    for out in (k_out, v_out):
-        assert out.shape == (num_tokens, Hk, D) and out.dtype == torch.bfloat16
-        assert out.stride(-1) == 1 and out.stride(1) == D
+        v_out = v_cache.new_empty((num_tokens, Hk, D), dtype=_BF16)
+    k_stride, v_stride = k_out.stride(), v_out.stride()
+    assert k_out.shape == (num_tokens, Hk, D) and v_out.shape == (num_tokens, Hk, D)
+    assert k_out.dtype is _BF16 and v_out.dtype is _BF16
     if B == 0 or num_tokens == 0:
         return k_out, v_out
+    assert k_stride[1:] == (D, 1) and v_stride[1:] == (D, 1)
     _call(device, "nkv_load_kvcache_fp8", k_cache.data_ptr(), v_cache.data_ptr(),
           k_exp.data_ptr(), v_exp.data_ptr(), num_blocks, block_size, block_tables.data_ptr(),
-          block_tables.size(1), cu_seqlens.data_ptr(), B, num_tokens, k_out.data_ptr(),
-          k_out.stride(0), v_out.data_ptr(), v_out.stride(0), Hk, D)
+          max_blocks, cu_seqlens.data_ptr(), B, num_tokens, k_out.data_ptr(),
+          k_stride[0], v_out.data_ptr(), v_stride[0], Hk, D)
     return k_out, v_out
 
 
@@ -584,29 +598,32 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """
     device = _one_device("paged_decode_fp8", q, k_cache, v_cache, k_exp, v_exp, block_tables,
                          context_lens, out, workspace)
-    B, Hq, D = q.shape
+    q_shape, q_stride = q.shape, q.stride()
+    B, Hq, D = q_shape
     num_blocks, block_size, Hk, Dk = _check_cache8(k_cache, v_cache, k_exp, v_exp)
+    rows, max_blocks = block_tables.shape
     assert Dk == D and Hk > 0 and Hq % Hk == 0
-    assert q.dtype == torch.bfloat16 and q.stride(-1) == 1
-    assert block_tables.dtype == torch.int32 and context_lens.dtype == torch.int32
-    assert block_tables.dim() == 2 and block_tables.size(0) >= B
+    assert q.dtype is _BF16 and q_stride[2] == 1
+    assert block_tables.dtype is _INT32 and context_lens.dtype is _INT32 and rows >= B
     assert context_lens.numel() >= B and context_lens.is_contiguous()
     if not block_tables.is_contiguous():
         block_tables = block_tables.contiguous()
     if out is None:
-        out = torch.empty(B, Hq, D, dtype=torch.bfloat16, device=device)
-    assert out.shape == q.shape and out.dtype == torch.bfloat16
-    assert out.stride(-1) == 1 and out.stride(1) == D
+        out = q.new_empty(q_shape)
+        out_stride = Hq * D
+    else:
+        assert out.shape == q_shape and out.dtype is _BF16
+        out_stride, *inner = out.stride()
+        assert B == 0 or inner == [D, 1]
     if B == 0:
         return out
     if workspace is None:
-        workspace = torch.empty(decode_fp8_workspace_bytes(Hq, Hk), dtype=torch.uint8,
-                                device=device)
+        workspace = k_exp.new_empty(decode_fp8_workspace_bytes(Hq, Hk))
     assert workspace.is_contiguous()
-    _call(device, "nkv_paged_decode_fp8", q.data_ptr(), q.stride(0), q.stride(1),
+    _call(device, "nkv_paged_decode_fp8", q.data_ptr(), q_stride[0], q_stride[1],
           k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), num_blocks,
-          block_tables.data_ptr(), block_tables.size(1), context_lens.data_ptr(), out.data_ptr(),
-          out.stride(0), B, Hq, Hk, D, block_size, float(softmax_scale), workspace.data_ptr(),
+          block_tables.data_ptr(), max_blocks, context_lens.data_ptr(), out.data_ptr(),
+          out_stride, B, Hq, Hk, D, block_size, softmax_scale, workspace.data_ptr(),
           workspace.numel() * workspace.element_size())
     return out
 
@@ -616,25 +633,23 @@ def decode_fp8_workspace_bytes(num_q_heads: int, num_kv_heads: int) -> int:
 
 
 # ---------------------------------------------------------------- pages
-_MAX_PAGE_REGIONS = 256
-
-
 def _page_regions(caches, page_dim: int, num_pages: int | None,
-                  block_size: int | None) -> tuple[torch.Tensor | None, int, int | None]:
-    """The caches as nkv_page_region records: (host int64 [n, 6], n, num_pages).
+                  block_size: int | None) -> tuple[array | None, int | None, int, int | None]:
+    """The caches as nkv_page_region records: (the records, their address, how
+    many, num_pages).
 
     Each cache is contiguous, [*lead, num_pages, *page] with page_dim leading
     dims; with a block size a page is [block_size, Hk, D] (values) or
     [Hk, block_size] (exponent bytes)."""
-    rows = []
+    records = array("q")
     for c in caches:
-        assert c.is_contiguous() and 0 <= page_dim < c.dim()
+        shape = c.shape
+        assert c.is_contiguous() and 0 <= page_dim < len(shape)
         if num_pages is None:
-            num_pages = c.size(page_dim)
-        assert c.size(page_dim) == num_pages, "the caches differ in their number of pages"
+            num_pages = shape[page_dim]
+        assert shape[page_dim] == num_pages, "the caches differ in their number of pages"
         size = c.element_size()
-        lead = math.prod(c.shape[:page_dim])
-        page = c.shape[page_dim + 1:]
+        page = shape[page_dim + 1:]
         page_bytes = math.prod(page) * size
         if block_size is None:
             seg_bytes = token_bytes = page_bytes
@@ -646,32 +661,27 @@ def _page_regions(caches, page_dim: int, num_pages: int | None,
             assert len(page) == 2 and page[1] == block_size
             token_bytes = size
             seg_bytes = block_size * size
-        rows.append((c.data_ptr(), lead, num_pages * page_bytes, page_bytes, seg_bytes,
-                     token_bytes))
-    if not rows:
-        return None, 0, num_pages
-    return torch.tensor(rows, dtype=torch.int64), len(rows), num_pages
+        records.extend((c.data_ptr(), math.prod(shape[:page_dim]), num_pages * page_bytes,
+                        page_bytes, seg_bytes, token_bytes))
+    if not caches:
+        return None, None, 0, num_pages
+    return records, records.buffer_info()[0], len(caches), num_pages
 
 
-def _check_page_state(block_tables, context_lens, ref_counts) -> None:
-    for t in (block_tables, context_lens, ref_counts):
-        assert t is None or (t.dtype == torch.int32 and t.is_contiguous())
-    assert block_tables.dim() == 2
-    assert context_lens is None or context_lens.numel() == block_tables.size(0)
+def _check_page_state(block_tables, *others) -> tuple[int, int]:
+    """(rows, max_blocks) of a block table; every tensor int32 and contiguous."""
+    rows, max_blocks = block_tables.shape
+    assert block_tables.dtype is _INT32 and block_tables.is_contiguous()
+    for t in others:
+        assert t.dtype is _INT32 and t.is_contiguous()
+    return rows, max_blocks
 
 
-def _check_index(*tensors: torch.Tensor) -> int:
-    n = tensors[0].numel()
-    for t in tensors:
-        assert t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n
-    return n
-
-
-def _pages_workspace(device: torch.device, n: int, num_pages: int) -> torch.Tensor:
-    """Scratch of one page call, from torch's allocator (stream-ordered, and a
-    captured graph's own)."""
-    return torch.empty(int(_lib.load().nkv_pages_workspace_size(n, num_pages)), dtype=torch.uint8,
-                       device=device)
+def _pages_workspace(like: torch.Tensor, n: int, num_pages: int) -> tuple[torch.Tensor, int]:
+    """Scratch of one page call on `like`'s device, from torch's allocator
+    (stream-ordered, and a captured graph's own), and its size."""
+    size = int(_lib.load().nkv_pages_workspace_size(n, num_pages))
+    return like.new_empty(size, dtype=torch.uint8), size
 
 
 def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor, page_dim: int = 0) -> None:
@@ -683,15 +693,16 @@ def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor, page_dim: int = 0) 
     whose target is another pair's target or source, or outside the cache, is
     not copied and sets DEVERR_PAGES. Pairs (-1, -1) are padding.
     """
-    caches = list(caches)
     device = _one_device("copy_pages", src, dst, *caches)
-    n = _check_index(src, dst)
-    regions, count, num_pages = _page_regions(caches, page_dim, None, None)
+    n = src.numel()
+    assert src.dtype is _INT32 and dst.dtype is _INT32 and dst.numel() == n
+    assert src.is_contiguous() and dst.is_contiguous()
+    _keep, regions, count, num_pages = _page_regions(caches, page_dim, None, None)
     if n == 0 or count == 0:
         return
-    ws = _pages_workspace(device, n, 0)
-    _call(device, "nkv_copy_pages", regions.data_ptr(), count, num_pages, src.data_ptr(),
-          dst.data_ptr(), n, ws.data_ptr(), ws.numel())
+    ws, size = _pages_workspace(src, n, 0)
+    _call(device, "nkv_copy_pages", regions, count, num_pages, src.data_ptr(), dst.data_ptr(), n,
+          ws.data_ptr(), size)
 
 
 def fork_pages(caches, block_tables: torch.Tensor, context_lens: torch.Tensor,
@@ -705,29 +716,28 @@ def fork_pages(caches, block_tables: torch.Tensor, context_lens: torch.Tensor,
 
     block_tables [rows, max_blocks], context_lens [rows] and ref_counts
     [num_pages] (all int32) are updated in place; caches as copy_pages, each
-    page [block_size, Hk, D] or, for exponent bytes, [Hk, block_size].
-    Returns out_pages int32 [n]: the page that was taken, -1 if none was
-    needed, -2 if the fork was not made (a target that is named twice or is a
-    source, a row out of range, no free page: DEVERR_PAGES is set; or a
-    (-1, -1) padding pair).
+    page [block_size, Hk, D] or, for exponent bytes, [Hk, block_size]. At most
+    4096 forks per call. Returns out_pages int32 [n]: the page that was taken,
+    -1 if none was needed, -2 if the fork was not made (a target that is named
+    twice or is a source, a row out of range, no free page: DEVERR_PAGES is
+    set; or a (-1, -1) padding pair).
     """
-    caches = list(caches)
     device = _one_device("fork_pages", block_tables, context_lens, ref_counts, src_rows, dst_rows,
                          out_pages, *caches)
-    _check_page_state(block_tables, context_lens, ref_counts)
-    n = _check_index(src_rows, dst_rows)
-    num_pages = ref_counts.numel()
-    regions, count, _ = _page_regions(caches, page_dim, num_pages, block_size)
+    rows, max_blocks = _check_page_state(block_tables, context_lens, ref_counts, src_rows, dst_rows)
+    n, num_pages = src_rows.numel(), ref_counts.numel()
+    assert context_lens.numel() == rows and dst_rows.numel() == n
+    _keep, regions, count, _ = _page_regions(caches, page_dim, num_pages, block_size)
     if out_pages is None:
-        out_pages = torch.empty(n, dtype=torch.int32, device=device)
-    assert out_pages.dtype == torch.int32 and out_pages.is_contiguous() and out_pages.numel() == n
+        out_pages = src_rows.new_empty(n)
+    assert out_pages.dtype is _INT32 and out_pages.is_contiguous() and out_pages.numel() == n
     if n == 0:
         return out_pages
-    ws = _pages_workspace(device, n, 0)
-    _call(device, "nkv_fork_pages", _ptr(regions), count, num_pages, block_size,
-          block_tables.data_ptr(), block_tables.size(1), block_tables.size(0),
-          context_lens.data_ptr(), ref_counts.data_ptr(), src_rows.data_ptr(),
-          dst_rows.data_ptr(), n, out_pages.data_ptr(), ws.data_ptr(), ws.numel())
+    ws, size = _pages_workspace(src_rows, n, 0)
+    _call(device, "nkv_fork_pages", regions, count, num_pages, block_size,
+          block_tables.data_ptr(), max_blocks, rows, context_lens.data_ptr(),
+          ref_counts.data_ptr(), src_rows.data_ptr(), dst_rows.data_ptr(), n,
+          out_pages.data_ptr(), ws.data_ptr(), size)
     return out_pages
 
 
@@ -738,13 +748,14 @@ def free_pages(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_count
     length becomes 0; trim=True: the pages past context_lens, as after a
     compression that shortened the rows on the device."""
     device = _one_device("free_pages", block_tables, context_lens, ref_counts, rows)
-    _check_page_state(block_tables, context_lens, ref_counts)
-    n = _check_index(rows)
+    num_rows, max_blocks = _check_page_state(block_tables, context_lens, ref_counts, rows)
+    n = rows.numel()
+    assert context_lens.numel() == num_rows
     if n == 0:
         return
-    _call(device, "nkv_free_pages", block_tables.data_ptr(), block_tables.size(1),
-          block_tables.size(0), context_lens.data_ptr(), ref_counts.data_ptr(),
-          ref_counts.numel(), block_size, rows.data_ptr(), n, 1 if trim else 0)
+    _call(device, "nkv_free_pages", block_tables.data_ptr(), max_blocks, num_rows,
+          context_lens.data_ptr(), ref_counts.data_ptr(), ref_counts.numel(), block_size,
+          rows.data_ptr(), n, 1 if trim else 0)
 
 
 def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, page_dim: int = 0,
@@ -755,24 +766,22 @@ def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, 
     the i-th used page at or past n moves to the i-th free page before n in
     every cache tensor, and tables and counts follow (in place, or into the
     out tensors). Returns out_num_live, int32 [1]: n."""
-    caches = list(caches)
     device = _one_device("compact_pages", block_tables, ref_counts, out_block_tables,
                          out_ref_counts, out_num_live, *caches)
     if out_block_tables is None:
         out_block_tables = block_tables
     if out_ref_counts is None:
         out_ref_counts = ref_counts
-    _check_page_state(block_tables, None, ref_counts)
-    _check_page_state(out_block_tables, None, out_ref_counts)
-    assert out_block_tables.shape == block_tables.shape
-    assert out_ref_counts.numel() == ref_counts.numel()
     if out_num_live is None:
-        out_num_live = torch.empty(1, dtype=torch.int32, device=device)
-    assert out_num_live.dtype == torch.int32 and out_num_live.numel() == 1
+        out_num_live = ref_counts.new_empty(1)
+    rows, max_blocks = _check_page_state(block_tables, ref_counts, out_block_tables,
+                                         out_ref_counts, out_num_live)
     num_pages = ref_counts.numel()
-    regions, count, _ = _page_regions(caches, page_dim, num_pages, None)
-    ws = _pages_workspace(device, num_pages // 2, num_pages)
-    _call(device, "nkv_compact_pages", _ptr(regions), count, num_pages, block_tables.data_ptr(),
-          out_block_tables.data_ptr(), block_tables.numel(), ref_counts.data_ptr(),
-          out_ref_counts.data_ptr(), out_num_live.data_ptr(), ws.data_ptr(), ws.numel())
+    assert out_block_tables.shape == (rows, max_blocks)
+    assert out_ref_counts.numel() == num_pages and out_num_live.numel() == 1
+    _keep, regions, count, _ = _page_regions(caches, page_dim, num_pages, None)
+    ws, size = _pages_workspace(ref_counts, num_pages // 2, num_pages)
+    _call(device, "nkv_compact_pages", regions, count, num_pages, block_tables.data_ptr(),
+          out_block_tables.data_ptr(), rows * max_blocks, ref_counts.data_ptr(),
+          out_ref_counts.data_ptr(), out_num_live.data_ptr(), ws.data_ptr(), size)
     return out_num_live
