@@ -30,9 +30,14 @@
 // warp; at the end of a pair a merger warp joins their states while they go on.
 //
 // Arithmetic. e4m3 is exact in f16, so K and V go to the tensor cores as f16
-// (mma.sync m16n8k16, 32-bit accumulators; groups of 1 to 16 heads are too
-// narrow for 64-row tcgen05 tiles). Products are transposed, S^T = K Q^T and
-// O^T = V^T P^T: tokens and dims fill the 16 rows, the heads the 8 columns.
+// (mma.sync m16n8k16, 32-bit sums; groups of 1 to 16 heads are too narrow for
+// 64-row tcgen05 tiles). mma.sync takes e4m3 operands too, with sums as exact,
+// but rearranges them on every use (a warp's dependent products 52 cycles
+// apart, f16 24): with q and the weights split in two e4m3 terms instead of K
+// and V converted, 128 rows of 8 kv heads took 226 us for 192. Products are
+// transposed, S^T = K Q^T and O^T = V^T P^T: tokens and dims fill the 16 rows,
+// the heads the 8 columns; groups of 9 to 16 heads give the two consumer groups
+// eight each, and every tile to both.
 //   * q is scaled by the power of two that brings its row's maximum into
 //     [1, 2) and rounded to f16: 11 bits for a bf16's 8, so only elements
 //     below 2^-14 of the maximum lose any (at most 2^-25 of the maximum).
@@ -71,13 +76,13 @@ struct Decode8Shape {
   static_assert(G == 1 || G == 2 || G == 4 || G == 8 || G == 16, "padded group width");
   static_assert(NH == 1 || (NH == 2 && G <= 8), "kv heads of a tile");
   static constexpr int kTokens = kDecode8Tile / NH;  // tokens of a tile
-  static constexpr int kNT = G <= 8 ? 1 : 2;  // 8-head column tiles
-  static constexpr int kStages = NH * G <= 4 ? 6 : G <= 8 ? 5 : 4;
+  static constexpr int kWarpHeads = G <= 8 ? G : 8;  // q heads of a consumer warp
+  static constexpr int kStages = NH * G <= 4 ? 6 : 5;
   static constexpr int kQBytes = (NH * G < 4 ? 4 : NH * G) * 256;
   // [K][V][q rows][K exponents][V exponents], 1024-byte aligned
   static constexpr int kStageBytes = 2 * kDecode8TileBytes + kQBytes + 1024;
   // the warps' (O, m, l) of a pair, as many pairs as fit beside the ring
-  static constexpr int kStateFloats = kDecode8Warps * G * kDecode8ORow;
+  static constexpr int kStateFloats = kDecode8Warps * kWarpHeads * kDecode8ORow;
   static constexpr int kSlots = G <= 4 && !(G == 4 && NH == 1) ? 2 : 1;
   static constexpr int kBarOffset = kStages * kStageBytes + kSlots * kStateFloats * 4;
   static constexpr int kSmemBytes = kBarOffset + (2 * kStages + 2 * kSlots) * 8 + kStages * 16 + kSlots * 16 + 16 + 1024;
@@ -176,7 +181,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   using S = Decode8Shape<G, NH>;
   constexpr int kTokens = S::kTokens;
   constexpr int kStages = S::kStages;
-  constexpr int kNT = S::kNT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -242,17 +246,20 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int g = p.g;
   const float NEG_INF = -INFINITY;
   // Sum of the consumer warps' states of one of a tile's q heads, this lane's
-  // four dims: M, L, acc. With two kv heads a tile, every other pair of warps.
+  // four dims: M, L, acc. With two kv heads a tile, every other pair of warps;
+  // with more than eight heads, every other group of four.
   auto merge_row = [&](const float* st, int row, float& M, float& L, float4& acc) {
-    constexpr int kStates = kDecode8Warps / NH;
-    const int kvh = NH == 1 ? 0 : row / g;
-    const float* src = st + (NH == 1 ? row : 2 * kvh * G + row - kvh * g) * kDecode8ORow;
+    constexpr int kHeads = S::kWarpHeads;
+    constexpr int kStates = G > 8 ? 4 : kDecode8Warps / NH;
+    const int part = G > 8 ? row >> 3 : NH == 1 ? 0 : row / g;  // eight heads; or a kv head's
+    const int first = G > 8 ? part * 4 : part * 2;              // its first warp
+    const float* src = st + (first * kHeads + row - part * (G > 8 ? 8 : g)) * kDecode8ORow;
     auto of = [](int w) { return NH == 1 ? w : (w >> 1) * 4 + (w & 1); };
     float2 ml[kStates];
     M = NEG_INF;
 #pragma unroll
     for (int w = 0; w < kStates; ++w) {
-      ml[w] = *reinterpret_cast<const float2*>(src + of(w) * G * kDecode8ORow + 128);
+      ml[w] = *reinterpret_cast<const float2*>(src + of(w) * kHeads * kDecode8ORow + 128);
       M = fmaxf(M, ml[w].x);
     }
     L = 0.f;
@@ -260,7 +267,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
 #pragma unroll
     for (int w = 0; w < kStates; ++w) {
       const float f = ml[w].x == NEG_INF ? 0.f : fast_exp2(ml[w].x - M);
-      const float4 x = *reinterpret_cast<const float4*>(src + of(w) * G * kDecode8ORow + 4 * lane);
+      const float4 x = *reinterpret_cast<const float4*>(src + of(w) * kHeads * kDecode8ORow + 4 * lane);
       L += ml[w].y * f;
       acc.x += x.x * f;
       acc.y += x.y * f;
@@ -549,18 +556,20 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     for (int i = threadIdx.x; i < groups * p.rows * 16; i += kDecode8Warps * 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
   }
 
-  float o[8][kNT][4];  // O^T: dims 16 dm + 2 gid (+ 1 for [2], [3]), heads 8 nt + 2 tig (+ 1 for odd)
-  float m_run[kNT][2], l_run[kNT][2], w_run[kNT][2];
-  uint32_t qb[8][kNT][2];
-  float qs[kNT][2];
+  float o[8][4];  // O^T: dims 16 dm + 2 gid (+ 1 for [2], [3]), heads 2 tig (+ 1 for odd)
+  float m_run[2], l_run[2], w_run[2];
+  uint32_t qb[8][2];  // q's B fragments
+  float qs[2];
   int stage = 0;
   uint32_t phase = 0;
   uint32_t merges = 0;
-  uint32_t turn = warp >> 2;  // even: the tile is this group's
+  uint32_t turn = G > 8 ? 0u : warp >> 2;  // even: the tile is this group's
   // the warp's 32 rows of a tile: tokens tok_base .. of its kvh-th kv head
   const int row_base = (warp & 3) * 32;
   const int kvh = NH == 1 ? 0 : (warp & 3) >> 1;
   const int tok_base = row_base - kvh * kTokens;
+  const int head0 = G > 8 ? (warp >> 2) * 8 : 0;  // its first q head
+  const int heads = min(g - head0, S::kWarpHeads);
   while (true) {
     if (!mbar_wait_bounded(smem_u32(&full_bar[stage]), phase)) {
       *abort_flag = 1;
@@ -576,51 +585,48 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
 
     if (flags & kFirst) {
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
+      for (int dm = 0; dm < 8; ++dm) o[dm][0] = o[dm][1] = o[dm][2] = o[dm][3] = 0.f;
+      m_run[0] = m_run[1] = w_run[0] = w_run[1] = NEG_INF;
+      l_run[0] = l_run[1] = 0.f;
+      // q's B fragments: head gid, dims 16 kk + 4 tig .. + 3
+      uint2 raw[8];
+      float top = 0.f;
 #pragma unroll
-        for (int dm = 0; dm < 8; ++dm) o[dm][nt][0] = o[dm][nt][1] = o[dm][nt][2] = o[dm][nt][3] = 0.f;
-        m_run[nt][0] = m_run[nt][1] = w_run[nt][0] = w_run[nt][1] = NEG_INF;
-        l_run[nt][0] = l_run[nt][1] = 0.f;
-        // q's B fragments: head 8 nt + gid, dims 16 kk + 4 tig .. + 3
-        const int head = 8 * nt + gid;
-        uint2 raw[8];
-        float top = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          raw[kk] = make_uint2(0u, 0u);
-          if (head < g)
-            raw[kk] = *reinterpret_cast<const uint2*>(sp + 2 * kDecode8TileBytes + (kvh * g + head) * 256 + kk * 32 +
-                                                      tig * 8);
-          top = fmaxf(top, fmaxf(fmaxf(fabsf(__uint_as_float(raw[kk].x << 16)),
-                                       fabsf(__uint_as_float(raw[kk].x & 0xffff0000u))),
-                                 fmaxf(fabsf(__uint_as_float(raw[kk].y << 16)),
-                                       fabsf(__uint_as_float(raw[kk].y & 0xffff0000u)))));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-        const float down = __uint_as_float((254u - e) << 23);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          qb[kk][nt][0] = pack_f16x2(__uint_as_float(raw[kk].x << 16) * down,
-                                     __uint_as_float(raw[kk].x & 0xffff0000u) * down);
-          qb[kk][nt][1] = pack_f16x2(__uint_as_float(raw[kk].y << 16) * down,
-                                     __uint_as_float(raw[kk].y & 0xffff0000u) * down);
-        }
-        const float up = __uint_as_float(e << 23) * p.scale_log2;
-        qs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * tig);
-        qs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * tig + 4);
+      for (int kk = 0; kk < 8; ++kk) {
+        raw[kk] = make_uint2(0u, 0u);
+        if (gid < heads)
+          raw[kk] = *reinterpret_cast<const uint2*>(sp + 2 * kDecode8TileBytes + (kvh * g + head0 + gid) * 256 +
+                                                    kk * 32 + tig * 8);
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(__uint_as_float(raw[kk].x << 16)),
+                                     fabsf(__uint_as_float(raw[kk].x & 0xffff0000u))),
+                               fmaxf(fabsf(__uint_as_float(raw[kk].y << 16)),
+                                     fabsf(__uint_as_float(raw[kk].y & 0xffff0000u)))));
       }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+      const float down = __uint_as_float((254u - e) << 23);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        qb[kk][0] = pack_f16x2(__uint_as_float(raw[kk].x << 16) * down,
+                               __uint_as_float(raw[kk].x & 0xffff0000u) * down);
+        qb[kk][1] = pack_f16x2(__uint_as_float(raw[kk].y << 16) * down,
+                               __uint_as_float(raw[kk].y & 0xffff0000u) * down);
+      }
+      const float up = __uint_as_float(e << 23) * p.scale_log2;
+      qs[0] = __shfl_sync(0xffffffffu, up, 8 * tig);
+      qs[1] = __shfl_sync(0xffffffffu, up, 8 * tig + 4);
     }
 
-    if ((turn++ & 1u) == 0u && tok_base < valid) {
+    const bool mine = G > 8 || (turn++ & 1u) == 0u;
+    if (mine && tok_base < valid) {
       const uint32_t sK = smem_u32(sp);
       const uint32_t sV = sK + kDecode8TileBytes;
       const int mi = lane >> 3;
       const int lrow = row_base + (mi & 1) * 8 + (lane & 7);
       // ---- S^T = K Q^T: two 16-token tiles, 8 steps of 16 dims. All loads first
-      // (each waits for none of the others), even and odd pairs of steps in
-      // sums of their own.
+      // (each waits for none of the others), even and odd steps in sums of their
+      // own.
       uint32_t raw[2][4][4];  // [token tile][pair of 16-byte chunks]: tokens 0-7 / 8-15 of the first, of the second
 #pragma unroll
       for (int kp = 0; kp < 4; ++kp)
@@ -628,27 +634,20 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         for (int mt = 0; mt < 2; ++mt)
           ldsm_x4(sK + swz128(lrow + 16 * mt, 2 * kp + (mi >> 1)), raw[mt][kp][0], raw[mt][kp][1],
                   raw[mt][kp][2], raw[mt][kp][3]);
-      float s[2][kNT][4], s_odd[2][kNT][4];
+      float s[2][4], s_odd[2][4];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[mt][nt][c] = s_odd[mt][nt][c] = 0.f;
+        for (int c = 0; c < 4; ++c) s[mt][c] = s_odd[mt][c] = 0.f;
 #pragma unroll
       for (int kp = 0; kp < 4; ++kp) {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           const uint32_t(&r)[4] = raw[mt][kp];
-          const uint32_t a0 = e4m3x2_to_f16x2(r[0]), a2 = e4m3x2_hi_to_f16x2(r[0]);
-          const uint32_t a1 = e4m3x2_to_f16x2(r[1]), a3 = e4m3x2_hi_to_f16x2(r[1]);
-          const uint32_t c0 = e4m3x2_to_f16x2(r[2]), c2 = e4m3x2_hi_to_f16x2(r[2]);
-          const uint32_t c1 = e4m3x2_to_f16x2(r[3]), c3 = e4m3x2_hi_to_f16x2(r[3]);
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            mma_f16_16816(s[mt][nt], a0, a1, a2, a3, qb[2 * kp][nt][0], qb[2 * kp][nt][1]);
-            mma_f16_16816(s_odd[mt][nt], c0, c1, c2, c3, qb[2 * kp + 1][nt][0], qb[2 * kp + 1][nt][1]);
-          }
+          mma_f16_16816(s[mt], e4m3x2_to_f16x2(r[0]), e4m3x2_to_f16x2(r[1]), e4m3x2_hi_to_f16x2(r[0]),
+                        e4m3x2_hi_to_f16x2(r[1]), qb[2 * kp][0], qb[2 * kp][1]);
+          mma_f16_16816(s_odd[mt], e4m3x2_to_f16x2(r[2]), e4m3x2_to_f16x2(r[3]), e4m3x2_hi_to_f16x2(r[2]),
+                        e4m3x2_hi_to_f16x2(r[3]), qb[2 * kp + 1][0], qb[2 * kp + 1][1]);
         }
       }
       // ---- the rest of the tile into registers, then the stage goes back to the
@@ -673,81 +672,83 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
                         raw[mt][dp][2], raw[mt][dp][3]);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&empty_bar[stage]));
-      // ---- scores in log2 units, weights
-      uint32_t wb[2][kNT][2];  // the weights as B fragments (two tokens of a head)
+      // ---- scores in log2 units, running maxima
+      float mx[2] = {NEG_INF, NEG_INF}, wx[2] = {NEG_INF, NEG_INF};
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        float mx[2] = {NEG_INF, NEG_INF}, wx[2] = {NEG_INF, NEG_INF};
+      for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float v = (s[mt][nt][c] + s_odd[mt][nt][c]) * (ks[mt][c >> 1] * qs[nt][c & 1]);
-            if (partial && tok_base + 16 * mt + 8 * (c >> 1) + gid >= valid) v = NEG_INF;
-            s[mt][nt][c] = v;
-            mx[c & 1] = fmaxf(mx[c & 1], v);
-            wx[c & 1] = fmaxf(wx[c & 1], v + vk[mt][c >> 1]);
-          }
+        for (int c = 0; c < 4; ++c) {
+          float v = (s[mt][c] + s_odd[mt][c]) * (ks[mt][c >> 1] * qs[c & 1]);
+          if (partial && tok_base + 16 * mt + 8 * (c >> 1) + gid >= valid) v = NEG_INF;
+          s[mt][c] = v;
+          mx[c & 1] = fmaxf(mx[c & 1], v);
+          wx[c & 1] = fmaxf(wx[c & 1], v + vk[mt][c >> 1]);
         }
-        float m_use[2], w_use[2], w_scale[2];
+      }
+      float m_use[2], w_use[2], w_scale[2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-            wx[e] = fmaxf(wx[e], __shfl_xor_sync(0xffffffffu, wx[e], x));
-          }
-          const float m_new = fmaxf(m_run[nt][e], mx[e]);
-          const float w_new = fmaxf(w_run[nt][e], wx[e]);
-          m_use[e] = m_new == NEG_INF ? 0.f : m_new;
-          w_use[e] = w_new == NEG_INF ? 0.f : w_new;
-          l_run[nt][e] *= fast_exp2(m_run[nt][e] - m_use[e]);
-          w_scale[e] = fast_exp2(w_run[nt][e] - w_use[e]);
-          m_run[nt][e] = m_new;
-          w_run[nt][e] = w_new;
+        for (int x = 4; x < 32; x <<= 1) {
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+          wx[e] = fmaxf(wx[e], __shfl_xor_sync(0xffffffffu, wx[e], x));
         }
+        const float m_new = fmaxf(m_run[e], mx[e]);
+        const float w_new = fmaxf(w_run[e], wx[e]);
+        m_use[e] = m_new == NEG_INF ? 0.f : m_new;
+        w_use[e] = w_new == NEG_INF ? 0.f : w_new;
+        l_run[e] *= fast_exp2(m_run[e] - m_use[e]);
+        w_scale[e] = fast_exp2(w_run[e] - w_use[e]);
+        m_run[e] = m_new;
+        w_run[e] = w_new;
+      }
+      uint32_t wb[2][2];  // the weights as B fragments (two tokens of a head)
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          float w[4];
+      for (int mt = 0; mt < 2; ++mt) {
+        float w[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            l_run[nt][c & 1] += fast_exp2(s[mt][nt][c] - m_use[c & 1]);
-            w[c] = fast_exp2(s[mt][nt][c] + vk[mt][c >> 1] - w_use[c & 1]);
-          }
-          wb[mt][nt][0] = movmatrix_trans(pack_f16x2(w[0], w[1]));
-          wb[mt][nt][1] = movmatrix_trans(pack_f16x2(w[2], w[3]));
+        for (int c = 0; c < 4; ++c) {
+          l_run[c & 1] += fast_exp2(s[mt][c] - m_use[c & 1]);
+          w[c] = fast_exp2(s[mt][c] + vk[mt][c >> 1] - w_use[c & 1]);
         }
+        wb[mt][0] = movmatrix_trans(pack_f16x2(w[0], w[1]));
+        wb[mt][1] = movmatrix_trans(pack_f16x2(w[2], w[3]));
+      }
+      // the maxima seldom move after the first tiles
+      if (__any_sync(0xffffffffu, w_scale[0] != 1.f || w_scale[1] != 1.f)) {
 #pragma unroll
         for (int dm = 0; dm < 8; ++dm) {
-          o[dm][nt][0] *= w_scale[0];
-          o[dm][nt][1] *= w_scale[1];
-          o[dm][nt][2] *= w_scale[0];
-          o[dm][nt][3] *= w_scale[1];
+          o[dm][0] *= w_scale[0];
+          o[dm][1] *= w_scale[1];
+          o[dm][2] *= w_scale[0];
+          o[dm][3] *= w_scale[1];
+        }
+      }
+      if (partial) {  // V of tokens past the end counts as 0
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const int tk = tok_base + 16 * mt + 2 * tig;
+          const uint32_t keep_lo = (tk < valid ? 0x0000ffffu : 0u) | (tk + 1 < valid ? 0xffff0000u : 0u);
+          const uint32_t keep_hi = (tk + 8 < valid ? 0x0000ffffu : 0u) | (tk + 9 < valid ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int dp = 0; dp < 4; ++dp) {
+            raw[mt][dp][0] &= keep_lo;
+            raw[mt][dp][1] &= keep_hi;
+            raw[mt][dp][2] &= keep_lo;
+            raw[mt][dp][3] &= keep_hi;
+          }
         }
       }
       // ---- O^T += V^T P^T: two steps of 16 tokens, 8 tiles of 16 dims
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;  // V of tokens past the end counts as 0
-        if (partial) {
-          const int tk = tok_base + 16 * mt + 2 * tig;
-          keep_lo = (tk < valid ? 0x0000ffffu : 0u) | (tk + 1 < valid ? 0xffff0000u : 0u);
-          keep_hi = (tk + 8 < valid ? 0x0000ffffu : 0u) | (tk + 9 < valid ? 0xffff0000u : 0u);
-        }
 #pragma unroll
-        for (int dp = 0; dp < 4; ++dp) {
-          const uint32_t(&r)[4] = raw[mt][dp];
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            // bytes: token 2 tig dims 2 gid, 2 gid + 1, token 2 tig + 1 the same
-            const uint32_t lo = __byte_perm(r[2 * half] & keep_lo, 0u, 0x3120);
-            const uint32_t hi = __byte_perm(r[2 * half + 1] & keep_hi, 0u, 0x3120);
-            const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_hi_to_f16x2(lo);
-            const uint32_t a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_hi_to_f16x2(hi);
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-              mma_f16_16816(o[2 * dp + half][nt], a0, a1, a2, a3, wb[mt][nt][0], wb[mt][nt][1]);
-          }
+        for (int dm = 0; dm < 8; ++dm) {
+          // bytes: token 2 tig dims 2 gid, 2 gid + 1, token 2 tig + 1 the same
+          const uint32_t lo = __byte_perm(raw[mt][dm >> 1][2 * (dm & 1)], 0u, 0x3120);
+          const uint32_t hi = __byte_perm(raw[mt][dm >> 1][2 * (dm & 1) + 1], 0u, 0x3120);
+          mma_f16_16816(o[dm], e4m3x2_to_f16x2(lo), e4m3x2_hi_to_f16x2(lo), e4m3x2_to_f16x2(hi),
+                        e4m3x2_hi_to_f16x2(hi), wb[mt][0], wb[mt][1]);
         }
       }
     } else {
@@ -767,23 +768,19 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       break;
     }
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
+    for (int e = 0; e < 2; ++e) {
+      float l = l_run[e];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float l = l_run[nt][e];
+      for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+      const int head = 2 * tig + e;
+      if (head < heads) {
+        const float m = m_run[e];
+        const float f = m == NEG_INF ? 0.f : fast_exp2(w_run[e] - m);
+        float* dst = state + slot * S::kStateFloats + (warp * S::kWarpHeads + head) * kDecode8ORow;
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-        const int head = 8 * nt + 2 * tig + e;
-        if (head < g) {
-          const float m = m_run[nt][e];
-          const float f = m == NEG_INF ? 0.f : fast_exp2(w_run[nt][e] - m);
-          float* dst = state + slot * S::kStateFloats + (warp * G + head) * kDecode8ORow;
-#pragma unroll
-          for (int dm = 0; dm < 8; ++dm)
-            *reinterpret_cast<float2*>(dst + 16 * dm + 2 * gid) =
-                make_float2(o[dm][nt][e] * f, o[dm][nt][2 + e] * f);
-          if (gid == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(m, l);
-        }
+        for (int dm = 0; dm < 8; ++dm)
+          *reinterpret_cast<float2*>(dst + 16 * dm + 2 * gid) = make_float2(o[dm][e] * f, o[dm][2 + e] * f);
+        if (gid == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(m, l);
       }
     }
     if (!kCluster && threadIdx.x == 0) {
