@@ -31,7 +31,7 @@ from itertools import chain
 import numpy as np
 import torch
 
-from ..utils.context import set_context
+from ..utils.context import get_context, set_context
 from .compress_schedule import padded_block_tables
 
 
@@ -107,4 +107,5 @@ class StepMetadata:
             context_lens, cu_q, cu_k = None, t(self.cu_seqlens_q), t(self.cu_seqlens_k)
         set_context(all_decode, cu_q, cu_k, self.max_seqlen_q, self.max_seqlen_k, slot_mapping,
                     context_lens, block_tables)
+        get_context().total_seqlen_k = int(self.cu_seqlens_k[-1])
         return input_ids, positions, logits_indices

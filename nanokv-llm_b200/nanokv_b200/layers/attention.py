@@ -15,6 +15,12 @@ nanokvllm/layers/attention.py:42-108, same order of work per layer:
 On a decode step that does not compress, 1 and 3 run as one launch
 (nkv_decode_step), which writes each kv head's new row right before reading
 that tile.
+
+With an 8-bit cache (k_cache / v_cache float8_e4m3fn, and k_exp / v_exp, their
+exponent bytes, set beside them) the rows are stored by nkv_store_kvcache_fp8
+and decode is nkv_paged_decode_fp8; a prompt chunk over a cached prefix reads
+its sequences back in bf16 (nkv_load_kvcache_fp8) and attends over them. The
+compressions work on a bf16 cache only and are refused.
 """
 
 from __future__ import annotations
@@ -37,6 +43,7 @@ class Attention(nn.Module):
         self.scale = scale
         self.num_kv_heads = num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
+        self.k_exp = self.v_exp = None  # exponent bytes of an 8-bit cache
         self.kv_compress_enabled = vllm_config.kv_compress_enabled
         if self.kv_compress_enabled:
             self.num_layers = num_layers
@@ -54,6 +61,13 @@ class Attention(nn.Module):
         q_norm / k_norm / rotary_emb followed by forward(q, k, v, Layer)."""
         context = get_context()
         k_cache, v_cache = self.k_cache, self.v_cache
+        if k_cache.dtype == torch.float8_e4m3fn:
+            q, v, k = ops.qk_norm_rope_store(
+                qkv, positions, cos_sin_cache, q_norm_weight, k_norm_weight, eps, self.num_heads,
+                self.num_kv_heads,
+                k_out=torch.empty(qkv.size(0), self.num_kv_heads, self.head_dim, dtype=qkv.dtype,
+                                  device=qkv.device))
+            return self._attend_fp8(q, k, v)
         has_cache = bool(k_cache.numel() and v_cache.numel())
         q, v, k = ops.qk_norm_rope_store(
             qkv, positions, cos_sin_cache, q_norm_weight, k_norm_weight, eps, self.num_heads,
@@ -66,7 +80,28 @@ class Attention(nn.Module):
         return self._attend(q, k, v, Layer, stored=has_cache)
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, Layer):
+        if self.k_cache.dtype == torch.float8_e4m3fn:
+            return self._attend_fp8(q, k, v)
         return self._attend(q, k, v, Layer, stored=False)
+
+    def _attend_fp8(self, q, k, v):
+        context = get_context()
+        cache = (self.k_cache, self.v_cache, self.k_exp, self.v_exp)
+        if self.kv_compress_enabled and context.is_compress_step:
+            raise ValueError("KV compression needs a bf16 cache")
+        if self.k_cache.numel():
+            ops.store_kvcache_fp8(k, v, *cache, context.slot_mapping)
+        if context.use_decode_kernel:
+            return ops.paged_decode_fp8(q, *cache, context.block_tables, context.context_lens,
+                                        self.scale).unsqueeze(1)
+        if context.block_tables is not None:  # keys come from the paged cache
+            tokens = context.total_seqlen_k or int(context.cu_seqlens_k[-1])
+            k, v = ops.load_kvcache_fp8(*cache, context.block_tables, context.cu_seqlens_k, tokens)
+        return ops.flash_attn_varlen_func(q, k, v, max_seqlen_q=context.max_seqlen_q,
+                                          cu_seqlens_q=context.cu_seqlens_q,
+                                          max_seqlen_k=context.max_seqlen_k,
+                                          cu_seqlens_k=context.cu_seqlens_k,
+                                          softmax_scale=self.scale, causal=True)
 
     def _attend(self, q, k, v, Layer, stored: bool):
         context = get_context()

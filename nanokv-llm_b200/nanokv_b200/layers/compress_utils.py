@@ -26,6 +26,14 @@ def _selected_tensor(context, device) -> torch.Tensor:
     return t
 
 
+def _free_pages(context, selected: torch.Tensor, block_size: int) -> None:
+    """The pages past the selected rows' new lengths, freed on the device when
+    the Context carries the pages' reference counts."""
+    if context.page_ref_counts is not None:
+        ops.free_pages(context.block_tables, context.context_lens, context.page_ref_counts,
+                       selected, block_size, trim=True)
+
+
 def MyCompressCompact(q_current: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       layer_id: int, block_size: int, window_blocks: int, keep_blocks: int,
                       keep_extra_tokens: int, num_layers: int, context=None) -> bool:
@@ -83,6 +91,7 @@ def MyCompressCompact(q_current: torch.Tensor, k_cache: torch.Tensor, v_cache: t
                 "freed_block_ids": freed,
                 "tail_uncompressed_len_after": 0,
             })
+        _free_pages(context, sel, B)
     return True
 
 
@@ -112,6 +121,8 @@ def _compress_device_selected(q_current, k_cache, v_cache, layer_id, block_size,
                           out_base_lens=base)
     ops.window_compress(q_current, k_cache, v_cache, context.block_tables, base,
                         context.context_lens, sel, window_blocks, keep_tokens, obs_window=1)
-    if layer_id + 1 >= num_layers and context.compress_selected_host is not None:
-        context.compress_selected_host.copy_(sel, non_blocking=True)
+    if layer_id + 1 >= num_layers:
+        if context.compress_selected_host is not None:
+            context.compress_selected_host.copy_(sel, non_blocking=True)
+        _free_pages(context, sel, B)
     return True

@@ -186,6 +186,7 @@ def decode_step(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_cache
     assert key.shape == (B, Hk, D) and value.shape == (B, Hk, D)
     assert key.stride(-1) == 1 and value.stride(-1) == 1
     assert key.stride(1) == D and value.stride(1) == D
+    assert k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16
     assert q.stride(-1) == 1 and k_cache.is_contiguous() and v_cache.is_contiguous()
     assert slot_mapping.dtype == torch.int32 and slot_mapping.numel() == B
     assert block_tables.dtype == torch.int32 and context_lens.dtype == torch.int32
@@ -268,6 +269,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, cos_sin_cache
     num_slots = 0
     if k_cache is not None:
         assert v_cache is not None and slot_mapping is not None
+        assert k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16
         assert k_cache.is_contiguous() and v_cache.is_contiguous() and v_cache.shape == k_cache.shape
         assert slot_mapping.dtype == torch.int32 and slot_mapping.numel() == T
         num_slots = k_cache.numel() // (num_kv_heads * D)
@@ -398,6 +400,7 @@ def window_compress(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if m == 0:
         return
     num_blocks, block_size, Hk, D = k_cache.shape
+    assert k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16
     Hq = q.size(1)
     assert q.stride(-1) == 1 and q.stride(1) == D
     assert selected.dtype == torch.int32 and selected.is_contiguous()
@@ -453,6 +456,7 @@ def threshold_compress(ring: torch.Tensor, ring_slot_of_selected: torch.Tensor, 
     slots, layers, W, Hq, D = ring.shape
     num_blocks, block_size, Hk, Dk = k_cache.shape
     assert Dk == D and ring.is_contiguous() and block_tables.is_contiguous()
+    assert k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
     if out_importance is not None:

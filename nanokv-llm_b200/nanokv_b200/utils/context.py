@@ -17,6 +17,13 @@ Additions, all optional and defaulting to "not provided":
                              device index tensors of the KvChat query window
                              (per active row, and per batch row for the fused
                              decode step)
+  total_seqlen_k             cu_seqlens_k[-1] on the host (0 = not provided), so
+                             that reading an 8-bit cache back needs no
+                             device->host sync
+  page_ref_counts            int32 [num_pages] device tensor: a periodic
+                             compression step then frees the pages that its
+                             rows no longer reach on the device
+                             (ops.free_pages), block_tables included
   compress_device_select, compress_topk, compress_tail_uncompressed_t,
   compress_selected_host     selection of a periodic compression step on the
                              device, so the step can be replayed from a CUDA
@@ -68,6 +75,9 @@ class Context:
     q_window_pos_t: torch.Tensor | None = None
     q_window_row_slot_t: torch.Tensor | None = None
     q_window_row_pos_t: torch.Tensor | None = None
+
+    total_seqlen_k: int = 0
+    page_ref_counts: torch.Tensor | None = None
 
     # device-side selection of a periodic compression step (graph-capturable):
     # the layers select at layer 0 into compress_selected_t ([topk], -1
