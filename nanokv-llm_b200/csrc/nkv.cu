@@ -1304,15 +1304,18 @@ int check_cache8(const void* k_cache, const void* v_cache, const void* k_exp, co
   return NKV_OK;
 }
 
-// A store or read-back of `tokens` tokens: 8 rounds of a CTA's rows where there
-// are enough for sixteen CTAs an SM, fewer to spread a short call. (With four
-// CTAs an SM, one wave, 33k tokens of 8 kv heads were read back in 58 instead
-// of 52 us.)
-int launch_rows8(void (*kernel)(nkv::Rows8Params), nkv::Rows8Params p, int64_t tokens, void* stream) {
+// A store or read-back of `tokens` tokens over ctas_per_sm CTAs an SM, or more
+// where a CTA would get more tokens than it holds. The store takes 4, one wave
+// whose CTAs run several rounds (18.8k tokens of 8 kv heads: 24.6 us, with 16
+// 27.0); the read-back, whose CTAs start with a chain of loads for their tokens,
+// 16 that overlap it (33.3k tokens: 43.4 us, with 4 48.3).
+int launch_rows8(void (*kernel)(nkv::Rows8Params), nkv::Rows8Params p, int64_t tokens,
+                 int ctas_per_sm, void* stream) {
   if (tokens * 2 * p.num_kv_heads > 0x7fffffff) return NKV_ERR_UNSUPPORTED;
   int dev = 0;
   cudaGetDevice(&dev);
-  const int64_t spread = (tokens + sm_count(dev) * 16 - 1) / (sm_count(dev) * 16);
+  const int64_t ctas_wanted = static_cast<int64_t>(sm_count(dev)) * ctas_per_sm;
+  const int64_t spread = (tokens + ctas_wanted - 1) / ctas_wanted;
   const int64_t most = std::max<int64_t>(1, nkv::kLoad8Tokens / p.num_kv_heads);
   p.num_tokens = static_cast<int>(tokens);
   p.cta_tokens = static_cast<int>(std::min(spread, most));
@@ -1514,7 +1517,7 @@ int nkv_store_kvcache_fp8(const void* key, int64_t key_stride, const void* value
   p.src_stride[0] = key_stride;
   p.src_stride[1] = value_stride;
   p.slot_mapping = slot_mapping;
-  return launch_rows8(nkv::store_kvcache_fp8_kernel, p, num_tokens, stream);
+  return launch_rows8(nkv::store_kvcache_fp8_kernel, p, num_tokens, 4, stream);
 }
 
 int nkv_load_kvcache_fp8(const void* k_cache, const void* v_cache, const void* k_exp,
@@ -1549,7 +1552,7 @@ int nkv_load_kvcache_fp8(const void* k_cache, const void* v_cache, const void* k
   p.cu_seqlens = cu_seqlens;
   p.max_blocks = max_blocks;
   p.batch = batch;
-  return launch_rows8(nkv::load_kvcache_fp8_kernel, p, num_tokens, stream);
+  return launch_rows8(nkv::load_kvcache_fp8_kernel, p, num_tokens, 16, stream);
 }
 
 size_t nkv_paged_decode_fp8_workspace_size(int32_t num_q_heads, int32_t num_kv_heads) {
