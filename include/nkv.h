@@ -436,7 +436,8 @@ int nkv_paged_decode_static_scratch(const void* q, int64_t q_stride_token, int64
 /* and k the smallest integer with a <= 448 * 2^k, kept in [-117, 119]       */
 /* (a == 0: -117), byte = k + 127 and value_j = e4m3(x_j * 2^-k) rounded to  */
 /* nearest even; an infinity becomes +-448, a NaN stays one. key / value     */
-/* rows as nkv_store_kvcache (strides in elements, multiples of 8).          */
+/* rows as nkv_store_kvcache (strides in elements, multiples of 8). Two      */
+/* tokens of one call must not name the same slot.                           */
 int nkv_store_kvcache_fp8(const void* key, int64_t key_stride, const void* value,
                           int64_t value_stride, void* k_cache, void* v_cache, void* k_exp,
                           void* v_exp, int64_t num_blocks, int32_t block_size,

@@ -68,8 +68,9 @@ __device__ __forceinline__ void page_share(const PageTables& t, const PageMove* 
   const int j = static_cast<int>(e - static_cast<int64_t>(i) * t.max_blocks);
   if (j >= moves[i].shared) return;
   const int32_t page = t.in[static_cast<int64_t>(t.src_rows[i]) * t.max_blocks + j];
-  if (page >= 0 && page < t.num_pages) atomicAdd(t.ref_counts + page, 1);
-  else raise_error(NKV_DEVERR_PAGES);
+  // a page of the source that nobody holds, or none of the cache, is flagged
+  if (page < 0 || page >= t.num_pages || atomicAdd(t.ref_counts + page, 1) <= 0)
+    raise_error(NKV_DEVERR_PAGES);
   t.out[static_cast<int64_t>(t.dst_rows[i]) * t.max_blocks + j] = page;
 }
 

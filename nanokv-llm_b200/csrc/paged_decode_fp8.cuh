@@ -85,7 +85,7 @@ struct Decode8Shape {
   static constexpr int kStateFloats = kDecode8Warps * kWarpHeads * kDecode8ORow;
   static constexpr int kSlots = G <= 4 && !(G == 4 && NH == 1) ? 2 : 1;
   static constexpr int kBarOffset = kStages * kStageBytes + kSlots * kStateFloats * 4;
-  static constexpr int kSmemBytes = kBarOffset + (2 * kStages + 2 * kSlots) * 8 + kStages * 16 + kSlots * 16 + 16 + 1024;
+  static constexpr int kSmemBytes = kBarOffset + (2 * kStages + 2 * kSlots) * 8 + kStages * 16 + kSlots * 16 + 32 + 1024;
 };
 
 // What CTA c leaves for the join: the pair that begins in its range and goes
@@ -191,9 +191,9 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   uint64_t* state_full = empty_bar + kStages;  // per slot: written by all consumer warps
   uint64_t* state_empty = state_full + kSlots;  // and read again
   // per stage: row (-1: no more tiles), head, flags | valid tokens << 8; per slot the same
-  int* meta = reinterpret_cast<int*>(state_empty + kSlots);
-  int* slot_meta = meta + kStages * 4;
-  volatile int* abort_flag = slot_meta + kSlots * 4;
+  int4* meta = reinterpret_cast<int4*>(smem + (S::kBarOffset + (2 * kStages + 2 * kSlots) * 8 + 15) / 16 * 16);
+  int4* slot_meta = meta + kStages;
+  volatile int* abort_flag = reinterpret_cast<int*>(slot_meta + kSlots);
   __shared__ int warp_tiles[kDecode8Merger + 1];
   __shared__ int first_row[2];  // the range's first row; its tiles in the rows before
   enum { kFirst = 1, kLast = 2, kPartial = 4, kPartialSlot1 = 8, kFinal = 16 };
@@ -349,7 +349,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         *abort_flag = 1;
         return;
       }
-      const int b = slot_meta[slot * 4], h = slot_meta[slot * 4 + 1], flags = slot_meta[slot * 4 + 2];
+      const int4 sm = slot_meta[slot];
+      const int b = sm.x, h = sm.y, flags = sm.z;
       if (b < 0 || (flags & kFinal)) return;
 #pragma unroll 2
       for (int row = 0; row < p.rows; ++row) put_row(slot, b, h, flags, row);
@@ -476,10 +477,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
             const uint32_t bar = smem_u32(&full_bar[stage]);
             if (at == 0) {
               if (for_k) {
-                int* m = meta + stage * 4;
-                m[0] = b;
-                m[1] = h;
-                m[2] = seg_flags | (j == 0 ? kFirst : 0) | (j == count - 1 ? kLast : 0) | (valid << 8);
+                meta[stage] =
+                    make_int4(b, h, seg_flags | (j == 0 ? kFirst : 0) | (j == count - 1 ? kLast : 0) | (valid << 8), 0);
               }
               const unsigned with_exps = (good >> first) & (0xffu >> (8 - boxes));
               mbar_arrive_expect_tx(bar, (((boxes * 128u + __popc(with_exps)) * NH) << box_shift) +
@@ -534,7 +533,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     if (lane == 0) {
       if (for_k && !kCluster) p.splits[blockIdx.x] = split;
       if (ok && wait_empty()) {
-        if (for_k) meta[stage * 4] = -1;
+        if (for_k) meta[stage].x = -1;
         mbar_arrive(smem_u32(&full_bar[stage]));
       } else {
         *abort_flag = 1;
@@ -575,10 +574,9 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       *abort_flag = 1;
       break;
     }
-    const int b = meta[stage * 4];
+    const int4 tile = meta[stage];
+    const int b = tile.x, h = tile.y, flags = tile.z;
     if (b < 0) break;
-    const int h = meta[stage * 4 + 1];
-    const int flags = meta[stage * 4 + 2];
     const int valid = flags >> 8;
     const uint8_t* sp = smem + stage * S::kStageBytes;
     const uint8_t* sexp = sp + 2 * kDecode8TileBytes + S::kQBytes;
@@ -784,9 +782,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       }
     }
     if (!kCluster && threadIdx.x == 0) {
-      slot_meta[slot * 4] = b;
-      slot_meta[slot * 4 + 1] = h;
-      slot_meta[slot * 4 + 2] = flags;
+      slot_meta[slot] = tile;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&state_full[slot]));
@@ -816,7 +812,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     // no tile fell to this CTA: the end marker for the merger
     const int slot = static_cast<int>(merges % kSlots);
     if (!mbar_wait_bounded(smem_u32(&state_empty[slot]), ((merges / kSlots) & 1u) ^ 1u)) *abort_flag = 1;
-    if (threadIdx.x == 0) slot_meta[slot * 4] = -1;
+    if (threadIdx.x == 0) slot_meta[slot].x = -1;
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&state_full[slot]));
     return;

@@ -2,6 +2,8 @@
 nkv_free_pages, nkv_compact_pages -- against plain loops (oracle/cache_pages.py).
 Everything is moved or counted, so every comparison is exact."""
 
+from collections import Counter
+
 import numpy as np
 import pytest
 import torch
@@ -170,6 +172,52 @@ def test_fork_refusals_and_an_empty_pool(cuda_lib):
     assert _deverr() == _lib().DEVERR_PAGES
 
 
+def test_fork_flags_a_page_that_nobody_holds(cuda_lib):
+    caches, pd = _caches(7, "views", 5, 16, 1)
+    t, n, r = _dev([[0, 3, -1], [-1, -1, -1]]), _dev([32, 0]), _dev([1, 1, 1, 0, 1])
+    assert _ops().fork_pages(caches, t, n, r, _dev([0]), _dev([1]), 16, page_dim=pd).tolist() == [-1]
+    assert _deverr() == _lib().DEVERR_PAGES
+
+
+def test_fork_of_many_rows_and_a_large_pool(cuda_lib):
+    """More forks and pages than the planning CTA has threads: 3,000 forks, the free pages past the first 16k."""
+    ops = _ops()
+    block, rows, width, pages = 16, 4000, 3, 21000
+    lens = [5 + (i % 40) for i in range(900)]
+    tables, row_lens, refs, used = _state(13, lens, rows, pages, block, width)
+    for p in range(16500):  # the low pages are taken by others
+        refs[p] = max(refs[p], 1)
+    caches, pd = _caches(14, "fp8", pages, block, 1)
+    free_rows = [r for r in range(rows) if r not in set(used)][:3000]
+    src = [used[i % len(used)] for i in range(3000)]
+    ref = _ref(tables, row_lens, refs, caches, pd, block)
+    t, n, r = _dev(tables), _dev(row_lens), _dev(refs)
+    # PageState counts repeats in a list: no repeats here, so its loops are kept short
+    ref_out = _fork_without_checks(ref, src, free_rows)
+    out = ops.fork_pages(caches, t, n, r, _dev(src), _dev(free_rows), block, page_dim=pd)
+    assert out.tolist() == ref_out
+    _same(ref, caches, pd, t, n, r)
+    assert _deverr() == 0
+
+
+def _fork_without_checks(ref, src, dst):
+    """PageState.fork for targets that are distinct and no sources."""
+    free = [p for p, r in enumerate(ref.refs) if r <= 0]
+    out = []
+    for s, d in zip(src, dst):
+        full, tail = divmod(ref.lens[s], ref.block)
+        page = free.pop(0) if tail else -1
+        for j in range(full):
+            ref.tables[d][j] = ref.tables[s][j]
+            ref.refs[ref.tables[s][j]] += 1
+        if tail:
+            ref.tables[d][full], ref.refs[page] = page, 1
+            ref.copy(ref.tables[s][full], page, tail)
+        ref.lens[d] = ref.lens[s]
+        out.append(page)
+    return out
+
+
 @pytest.mark.parametrize("trim", [False, True])
 @pytest.mark.parametrize("n_rows,block,width", [(3, 16, 5), (400, 64, 30), (9, 256, 700)])
 def test_free_pages(cuda_lib, n_rows, block, width, trim):
@@ -212,6 +260,7 @@ COMPACT = [
     (96, 23, 16, 32, 3),
     (1025, 400, 64, 16, 1),
     (5000, 2600, 300, 16, 1),
+    (40000, 17000, 500, 16, 1),
 ]
 
 
@@ -228,7 +277,8 @@ def test_compact_pages(cuda_lib, kind, in_place, pages, live, rows, block, Hk):
         tables[i % rows][i // rows] = p
         if i % 3 == 0:  # shared with another row
             tables[(i + 1) % rows][width - 1] = p
-    refs = [sum(row.count(p) for row in tables) for p in range(pages)]
+    held = Counter(p for row in tables for p in row)
+    refs = [held[p] for p in range(pages)]
     caches, pd = _caches(8, kind, pages, block, Hk, layers=1)
     ref = _ref(tables, [], refs, caches, pd, block)
     t, r = _dev(tables), _dev(refs)

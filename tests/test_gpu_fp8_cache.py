@@ -222,6 +222,8 @@ DECODE = [
     ([200] * 37, 24, 8, 384),
     (list(range(0, 300)), 2, 1, 128),
     ([128] * 400, 3, 3, 128),
+    ([(37 * i) % 41 for i in range(4099)], 4, 2, 16),
+    ([700, 0, 90000], 36, 4, 256),
 ]
 
 
@@ -263,6 +265,44 @@ def test_decode_queries_of_any_size(cuda_lib, factor):
     q = (_q(8, 2, 4).float() * factor).to(torch.bfloat16)
     out = _ops().paged_decode_fp8(q, *c.dev(), c.tables.to(DEV), c.lens_t(), SCALE)
     _check_decode(c, q, out)
+
+
+def test_decode_nan_and_infinity_among_the_live_rows(cuda_lib):
+    """A NaN among a row's keys, values or queries is its heads' result, nobody else's."""
+    c = Cache(15, [300, 300, 300, 40], 2, 64)
+    q = _q(15, 4, 4)
+    at = lambda b, t: (int(c.tables[b, t // 64]), t % 64)  # noqa: E731
+    c.k[(*at(0, 250), 0, 3)] = 0x7F
+    c.v[(*at(1, 7), 1, 5)] = 0xFF
+    q[2, 3, 9] = float("nan")
+    out = _ops().paged_decode_fp8(q, *c.dev(), c.tables.to(DEV), c.lens_t(), SCALE)
+    bad = torch.zeros(4, 4, 128, dtype=torch.bool, device=DEV)
+    bad[0, :2] = True
+    bad[1, 2:, 5] = True
+    bad[2, 3] = True
+    assert torch.equal(torch.isnan(out), bad)
+    c.k[(*at(0, 250), 0, 3)] = 0
+    c.v[(*at(1, 7), 1, 5)] = 0
+    clean = torch.where(torch.isnan(q), torch.zeros_like(q), q)
+    ref, bound = decode_fp8_ref(clean, *(t.to(DEV) for t in (c.k, c.v, c.ke, c.ve)), c.tables.to(DEV),
+                                c.lens_t(), SCALE)
+    good = ~bad.any(-1)  # heads that no NaN reaches
+    assert bool(((out.double() - ref).abs() <= bound)[good].all())
+
+
+def test_decode_without_tables(cuda_lib):
+    """No page at all: every row is empty, or flagged and empty."""
+    from nanokv_b200 import _lib
+
+    c = Cache(16, [0, 0, 0], 2, 64)
+    q = _q(16, 3, 4)
+    tables = torch.empty(3, 0, dtype=torch.int32, device=DEV)
+    out = torch.full((3, 4, 128), 3.0, dtype=torch.bfloat16, device=DEV)
+    _ops().paged_decode_fp8(q, *c.dev(), tables, c.lens_t(), SCALE, out=out)
+    assert bool((out == 0).all()) and _deverr() == 0
+    out.fill_(3.0)
+    _ops().paged_decode_fp8(q, *c.dev(), tables, c.lens_t() + 5, SCALE, out=out)
+    assert bool((out == 0).all()) and _deverr() == _lib.DEVERR_DECODE_BLOCK
 
 
 def test_decode_strided_rows_and_outputs(cuda_lib):
