@@ -195,7 +195,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   int4* slot_meta = meta + kStages;
   volatile int* abort_flag = reinterpret_cast<int*>(slot_meta + kSlots);
   __shared__ int warp_tiles[kDecode8Merger + 1];
-  __shared__ int first_row[2];  // the range's first row; its tiles in the rows before
+  __shared__ int4 first_tile;  // the range's first row, tile of it, the row's length and tiles
   enum { kFirst = 1, kLast = 2, kPartial = 4, kPartialSlot1 = 8, kFinal = 16 };
 
   const int warp = threadIdx.x >> 5;
@@ -279,7 +279,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   // ---- the call's tiles and this CTA's range of them (the split form). Every
   // thread sums the tiles of a few rows in turn; the one whose rows hold the
   // range's first tile finds the row.
-  int total = 0, head_tiles = 0, ctas = 1, u = 0, left = 0;
+  int total = 0, head_tiles = 0, ctas = 1, u = 0, left = 0, head_first = 0;
   if constexpr (!kCluster) {
     const int per = (p.batch + static_cast<int>(blockDim.x) - 1) / static_cast<int>(blockDim.x);
     const int row0 = min(static_cast<int>(threadIdx.x) * per, p.batch), row1 = min(row0 + per, p.batch);
@@ -309,16 +309,18 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       u = c * share + min(c, more);
       left = share + (c < more ? 1 : 0);
     }
-    const int rest = left > 0 ? u % head_tiles : 0;
+    head_first = left > 0 ? u / head_tiles : 0;
+    const int rest = u - head_first * head_tiles;
     if (mine > 0 && rest >= before && rest < before + mine) {
-      int at = before, i = row0;
-      for (;; ++i) {
-        const int n = decode8_tiles<NH>(decode8_length(p, i));
-        if (rest < at + n) break;
+      int at = before;
+      for (int i = row0;; ++i) {
+        const int len = decode8_length(p, i), n = decode8_tiles<NH>(len);
+        if (rest < at + n) {
+          first_tile = make_int4(i, rest - at, len, n);
+          break;
+        }
         at += n;
       }
-      first_row[0] = i;
-      first_row[1] = at;
     }
     __syncthreads();
   }
@@ -375,6 +377,9 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     const int box_shift = 31 - __clz(p.box_rows);
     const int tile_boxes = kTokens >> box_shift;
     const int page_boxes = p.block_size >> box_shift;
+    // of a page: a shift where it is a power of two (every usual size)
+    const int page_shift = (page_boxes & (page_boxes - 1)) == 0 ? 31 - __clz(page_boxes) : -1;
+    auto page_of = [&](int box) { return page_shift >= 0 ? box >> page_shift : box / page_boxes; };
     // ---- its first row, head and tile
     int b = 0, h = 0, t = 0, len = 0, ntiles = 0;
     if (kCluster) {
@@ -386,11 +391,12 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       t = rank * ntiles / csize;
       left = (rank + 1) * ntiles / csize - t;
     } else if (left > 0) {
-      b = first_row[0];
-      h = u / head_tiles;
-      t = u - h * head_tiles - first_row[1];
-      len = decode8_length(p, b);
-      ntiles = decode8_tiles<NH>(len);
+      const int4 at = first_tile;
+      b = at.x;
+      h = head_first;
+      t = at.y;
+      len = at.z;
+      ntiles = at.w;
     }
     // the lengths of 32 rows from lens0, one per lane
     int lens0 = -32, my_len = 0;
@@ -416,7 +422,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     };
     // the table entry of this lane's box, first + lane, of a row
     auto load_entry = [&](int row, int first) {
-      const int page = (first + lane) / page_boxes;
+      const int page = page_of(first + lane);
       return page < p.max_blocks
                  ? __ldg(p.block_tables + static_cast<int64_t>(row) * p.max_blocks + page)
                  : -1;
@@ -427,7 +433,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     auto set_window = [&](int first, int blk) {
       box0 = first;
       const bool ok = blk >= 0 && blk < p.num_blocks;
-      const int off = ((first + lane) % page_boxes) << box_shift;
+      const int off = (first + lane - page_of(first + lane) * page_boxes) << box_shift;
       // no page: rows far outside the tensor, which TMA fills with zeros
       slot = ok ? blk * p.block_size + off : -2 * kDecode8Tile;
       exp_src = exps + (static_cast<int64_t>(blk) * p.num_kv_heads + h * NH) * p.block_size + off;
