@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 import threading
 from array import array
+from functools import lru_cache
 
 import torch
 
@@ -489,7 +490,7 @@ def _call(device: int, name: str, *args) -> None:
     """Entry point `name` on the device's current stream, with that device current."""
     fn = getattr(_lib.load(), name)
     stream = torch._C._cuda_getCurrentRawStream(device)
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         status = fn(*args, stream)
     else:
         with torch.cuda.device(device):
@@ -571,7 +572,7 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.
     if k_out is None:
         k_out = k_cache.new_empty((num_tokens, Hk, D), dtype=_BF16)
     if v_out is None:
-        v_out = v_cache.new_empty((num_tokens, Hk, D), dtype=_BF16)
+        v_out = torch.empty_like(k_out, memory_format=torch.contiguous_format)
     k_stride, v_stride = k_out.stride(), v_out.stride()
     assert k_out.shape == (num_tokens, Hk, D) and v_out.shape == (num_tokens, Hk, D)
     assert k_out.dtype is _BF16 and v_out.dtype is _BF16
@@ -613,7 +614,7 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if not block_tables.is_contiguous():
         block_tables = block_tables.contiguous()
     if out is None:
-        out = q.new_empty(q_shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         out_stride = Hq * D
     else:
         assert out.shape == q_shape and out.dtype is _BF16
@@ -632,6 +633,7 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
+@lru_cache(maxsize=None)
 def decode_fp8_workspace_bytes(num_q_heads: int, num_kv_heads: int) -> int:
     return int(_lib.load().nkv_paged_decode_fp8_workspace_size(num_q_heads, num_kv_heads))
 
@@ -682,10 +684,15 @@ def _check_page_state(block_tables, *others) -> tuple[int, int]:
 
 
 def _pages_workspace(like: torch.Tensor, n: int, num_pages: int) -> tuple[torch.Tensor, int]:
-    """Scratch of one page call on `like`'s device, from torch's allocator
-    (stream-ordered, and a captured graph's own), and its size."""
-    size = int(_lib.load().nkv_pages_workspace_size(n, num_pages))
-    return like.new_empty(size, dtype=torch.uint8), size
+    """Scratch of one page call on the device of `like` (int32), from torch's
+    allocator (stream-ordered, and a captured graph's own), and its size."""
+    size = _pages_workspace_bytes(n, num_pages)
+    return like.new_empty(size // 4), size
+
+
+@lru_cache(maxsize=4096)
+def _pages_workspace_bytes(n: int, num_pages: int) -> int:
+    return int(_lib.load().nkv_pages_workspace_size(n, num_pages))
 
 
 def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor, page_dim: int = 0) -> None:
