@@ -1341,8 +1341,15 @@ int encode_cache8(CUtensorMap* map, const void* base, int num_kv_heads, int64_t 
   return r == CUDA_SUCCESS ? NKV_OK : NKV_ERR_ALIGNMENT;
 }
 
-// Most tiles per CTA of a cluster launch.
+// A cluster launch (C CTAs for each of P pairs of up to T tiles) ends about 3 us
+// before the two launches of the split form, and a CTA of it has T / C tiles
+// instead of P T / SMs: it is taken while that is at most 5 tiles more (one row
+// x 8 heads: 8,192 tokens 10.1 against 10.3 us, 16,384 15.6 against 13.0; x 1
+// head: 4,096 7.5 against 7.9, 8,192 10.0 against 8.6; 4 rows x 8: 8,192 16.5
+// against 18.9). And up to 12 tiles a CTA, because T comes from the table's
+// width: the split balances rows that are shorter.
 constexpr int kDecode8ClusterTiles = 12;
+constexpr int kDecode8ClusterMore = 5;
 
 // kv heads of a tile of the split form: two where they pair up (a token's 256
 // bytes of neighbouring heads are read together) and their q rows leave room
@@ -1469,12 +1476,10 @@ int launch_decode8(const Decode8Cache& c, const nkv::Decode8Params& p, cudaStrea
   const int sms = std::min(sm_count(dev), nkv::kDecode8MaxCtas);
   const int64_t row_tiles =
       (static_cast<int64_t>(p.max_blocks) * p.block_size + nkv::kDecode8Tile - 1) / nkv::kDecode8Tile;
-  // Clusters while every CTA of one gets few tiles: a longer row is better
-  // spread over all SMs (a cluster leaves some idle), a shorter one ends
-  // before the second kernel of the split would have started.
-  const int64_t cluster = std::min<int64_t>(
-      {nkv::kDecode8MaxCluster, row_tiles, sms / (p.batch * p.num_kv_heads)});
-  if (cluster > 1 && row_tiles <= cluster * kDecode8ClusterTiles) {
+  const int64_t pairs = p.batch * p.num_kv_heads;
+  const int64_t cluster = std::min<int64_t>({nkv::kDecode8MaxCluster, row_tiles, sms / pairs});
+  if (cluster > 1 && row_tiles <= cluster * kDecode8ClusterTiles &&
+      row_tiles * (sms - cluster * pairs) <= kDecode8ClusterMore * sms * cluster) {
     bool launched = false;
     const int st = launch_decode8_cluster<G>(c, p, static_cast<int>(cluster), stream, &launched);
     if (st != NKV_OK || launched) return st;
