@@ -1416,7 +1416,7 @@ int launch_decode8_cluster(const Decode8Cache& c, nkv::Decode8Params p, int max_
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   const int pairs = p.batch * p.num_kv_heads;
-  for (p.cluster = max_cluster; p.cluster > 1; --p.cluster) {
+  for (p.cluster = max_cluster; p.cluster >= 1; --p.cluster) {
     cfg.gridDim = dim3(pairs * p.cluster);
     attr[1].val.clusterDim.x = p.cluster;
     int& n = fit[dev][p.cluster];
@@ -1478,7 +1478,7 @@ int launch_decode8(const Decode8Cache& c, const nkv::Decode8Params& p, cudaStrea
       (static_cast<int64_t>(p.max_blocks) * p.block_size + nkv::kDecode8Tile - 1) / nkv::kDecode8Tile;
   const int64_t pairs = p.batch * p.num_kv_heads;
   const int64_t cluster = std::min<int64_t>({nkv::kDecode8MaxCluster, row_tiles, sms / pairs});
-  if (cluster > 1 && row_tiles <= cluster * kDecode8ClusterTiles &&
+  if (cluster >= 1 && row_tiles <= cluster * kDecode8ClusterTiles &&
       row_tiles * (sms - cluster * pairs) <= kDecode8ClusterMore * sms * cluster) {
     bool launched = false;
     const int st = launch_decode8_cluster<G>(c, p, static_cast<int>(cluster), stream, &launched);

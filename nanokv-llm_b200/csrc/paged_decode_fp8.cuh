@@ -113,7 +113,7 @@ struct Decode8Params {
   float scale_log2;
   __nv_bfloat16* out;
   int64_t out_stride_token;
-  int cluster;           // > 1: clusters of that many CTAs, one per (row, kv head), that join by themselves
+  int cluster;           // CTAs of a cluster, one cluster per (row, kv head) that joins by itself
   Decode8Split* splits;  // [CTAs]
   float* parts;          // [CTAs][2][rows][kDecode8ORow]: range's first pair, last pair
 };
