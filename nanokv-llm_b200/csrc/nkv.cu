@@ -1462,11 +1462,16 @@ int launch_decode8_split(const Decode8Cache& c, nkv::Decode8Params p, int sms, c
   const int64_t row_tiles = (static_cast<int64_t>(p.max_blocks) * p.block_size + S::kTokens - 1) / S::kTokens;
   const int grid = static_cast<int>(std::min<int64_t>(
       sms - even <= sms / 20 ? even : sms, std::max<int64_t>(1, row_tiles * p.batch * groups)));
+  // The join: a pair's q heads in one CTA where pairs are many and so have few
+  // pieces (16 q heads a pair, 128 rows: 33 against 36 us; 8: 17.4 against 18.2;
+  // 4, 400 rows: 18.2 against 17.5), a CTA each where few pairs have many (4 rows,
+  // 8 q heads: 42.7 against 45.0).
+  p.join_rows = p.rows > 4 && p.batch * groups >= grid / 4 ? p.rows : 1;
   st = launch_dependent(kernel, dim3(grid), dim3(nkv::kDecode8Threads<false>), S::kSmemBytes, stream,
                         tk, tv, p);
   if (st != NKV_OK || row_tiles <= 1 || grid == 1) return st;
-  return launch_dependent(nkv::decode_fp8_join_kernel, dim3(grid, p.rows),
-                          dim3(nkv::kDecode8JoinWarps * 32), 0, stream, p);
+  return launch_dependent(nkv::decode_fp8_join_kernel, dim3(grid, (p.rows + p.join_rows - 1) / p.join_rows),
+                          dim3(p.join_rows <= 8 ? 256 : nkv::kDecode8JoinWarps * 32), 0, stream, p);
 }
 
 template <int G>

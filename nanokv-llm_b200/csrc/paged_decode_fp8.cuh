@@ -68,7 +68,7 @@ constexpr int kDecode8Threads = (kDecode8Merger + (kCluster ? 0 : 1)) * 32;
 constexpr int kDecode8TileBytes = kDecode8Tile * 128;
 constexpr int kDecode8MaxCtas = 160;
 constexpr int kDecode8ORow = 132;   // floats of one row of a partial: O[128], m, l, 2 of padding
-constexpr int kDecode8JoinWarps = 8;
+constexpr int kDecode8JoinWarps = 16;  // at most; no fewer than the q heads of a tile
 constexpr int kDecode8MaxCluster = 8;
 
 template <int G, int NH>
@@ -110,6 +110,7 @@ struct Decode8Params {
   int num_kv_heads;
   int g;
   int rows;       // q heads of a tile's kv heads
+  int join_rows;  // of them, how many a CTA of the join takes
   float scale_log2;
   __nv_bfloat16* out;
   int64_t out_stride_token;
@@ -872,66 +873,72 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
 }
 
 // Joins the pieces of the pair that begins in CTA blockIdx.x's range and goes
-// on in later ones (row blockIdx.y of its q heads): each warp sums every eighth
-// piece, the first warp the eight sums, always in the same order.
+// on in later ones, join_rows of its q heads from join_rows * blockIdx.y on:
+// `parts` warps for each head, each summing every parts-th piece, then one of
+// them their sums, always in the same order.
 __global__ void __launch_bounds__(kDecode8JoinWarps * 32) decode_fp8_join_kernel(const Decode8Params p) {
   __shared__ float sums[kDecode8JoinWarps][kDecode8ORow];
   grid_dependency_wait();
   allow_dependent_launch();
   const Decode8Split split = p.splits[blockIdx.x];
   if (split.pieces == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y;
-  // piece 0 is the range's last pair of this CTA, piece i the first of CTA + i
-  auto piece = [&](int i) {
-    return p.parts + ((static_cast<int>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row) * kDecode8ORow;
-  };
-  // eight pieces' loads at a time, then one rescaling of the sums so far
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int parts = blockDim.x >> 5;
+  while (parts * p.join_rows > static_cast<int>(blockDim.x >> 5)) parts >>= 1;
+  const int in_cta = warp / parts, part = warp - in_cta * parts;
+  const int row = blockIdx.y * p.join_rows + in_cta;
+  const bool live = in_cta < p.join_rows && row < p.rows;
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = warp; i < split.pieces; i += 8 * kDecode8JoinWarps) {
-    float2 ml[8];
-    float4 x[8];
-    float top = M;
+  if (live) {
+    // piece 0 is the range's last pair of this CTA, piece i the first of CTA + i
+    auto piece = [&](int i) {
+      return p.parts + ((static_cast<int>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row) * kDecode8ORow;
+    };
+    // eight pieces' loads at a time, then one rescaling of the sums so far
+    for (int i = part; i < split.pieces; i += 8 * parts) {
+      float2 ml[8];
+      float4 x[8];
+      float top = M;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      ml[k] = make_float2(-INFINITY, 0.f);
-      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i + k * kDecode8JoinWarps < split.pieces) {
-        const float* src = piece(i + k * kDecode8JoinWarps);
-        ml[k] = *reinterpret_cast<const float2*>(src + 128);
-        x[k] = *reinterpret_cast<const float4*>(src + 4 * lane);
+      for (int k = 0; k < 8; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i + k * parts < split.pieces) {
+          const float* src = piece(i + k * parts);
+          ml[k] = *reinterpret_cast<const float2*>(src + 128);
+          x[k] = *reinterpret_cast<const float4*>(src + 4 * lane);
+        }
       }
-    }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
-    const float keep = M == -INFINITY ? 0.f : fast_exp2(M - top);
-    M = top;
-    L *= keep;
-    acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+      const float keep = M == -INFINITY ? 0.f : fast_exp2(M - top);
+      M = top;
+      L *= keep;
+      acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float f = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - top);
-      L += ml[k].y * f;
-      acc.x += x[k].x * f;
-      acc.y += x[k].y * f;
-      acc.z += x[k].z * f;
-      acc.w += x[k].w * f;
+      for (int k = 0; k < 8; ++k) {
+        const float f = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - top);
+        L += ml[k].y * f;
+        acc.x += x[k].x * f;
+        acc.y += x[k].y * f;
+        acc.z += x[k].z * f;
+        acc.w += x[k].w * f;
+      }
     }
   }
   *reinterpret_cast<float4*>(&sums[warp][4 * lane]) = acc;
   if (lane == 0) *reinterpret_cast<float2*>(&sums[warp][128]) = make_float2(M, L);
   __syncthreads();
-  if (warp != 0) return;
-  M = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kDecode8JoinWarps; ++w) M = fmaxf(M, sums[w][128]);
+  if (!live || part != 0) return;
+  for (int w = 1; w < parts; ++w) M = fmaxf(M, sums[warp + w][128]);
   L = 0.f;
   acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < kDecode8JoinWarps; ++w) {
-    const float f = sums[w][128] == -INFINITY ? 0.f : fast_exp2(sums[w][128] - M);
-    const float4 x = *reinterpret_cast<const float4*>(&sums[w][4 * lane]);
-    L += sums[w][129] * f;
+  for (int w = 0; w < parts; ++w) {
+    const float* src = sums[warp + w];
+    const float f = src[128] == -INFINITY ? 0.f : fast_exp2(src[128] - M);
+    const float4 x = *reinterpret_cast<const float4*>(src + 4 * lane);
+    L += src[129] * f;
     acc.x += x.x * f;
     acc.y += x.y * f;
     acc.z += x.z * f;
