@@ -9,19 +9,21 @@
 // FLOP, 2 g FLOP a byte.
 //
 // Split and join. The work of a call is the 128-token tiles of every (row, kv
-// head) pair in the order (head, row, tile); CTA c of n takes the tiles
-// [c T / n, (c + 1) T / n) (rounded: the first T mod n CTAs take one more). (Heads outermost: CTAs n / Hk apart then read the
-// same tokens of different heads at the same time, neighbours in memory.) Every CTA has the same number of tiles, whatever
-// the lengths, and which tiles depends on the lengths alone: results are the
-// same every time. A CTA finishes the pairs that lie inside its range; of a
-// pair that it shares with others it leaves the raw (m, l, O) in the workspace
+// head) pair (64 tokens of two heads where kv heads pair up) in the order (head,
+// row, tile); CTA c of n takes T / n of the T tiles, the first T mod n CTAs one
+// more. (Heads outermost: CTAs n / Hk apart then read the same tokens of
+// different heads at the same time, neighbours in memory.) The ranges are equal
+// whatever the lengths, and which tiles they hold depends on the lengths alone:
+// results are the same every time. A CTA finishes the pairs that lie inside its
+// range; of a pair that it shares with others it leaves the raw (m, l, O) in the workspace
 // (at most two: at its range's start and end), which a second kernel, launched
 // behind the first with programmatic dependence, joins in the CTAs' order. No
 // counters, so the workspace needs no content and outlives nothing.
 //
-// Small calls, whose time is latency, are launched as thread-block clusters
-// instead, one per (row, kv head): no scan of the lengths, and the CTAs' parts
-// are joined through distributed shared memory by the same kernel.
+// Calls of at most one (row, kv head) per SM whose time is latency are launched
+// as thread-block clusters of 1 to 8 CTAs instead, a cluster per (row, kv head):
+// no scan of the lengths and no second launch, the CTAs' parts are joined through
+// distributed shared memory by the same kernel.
 //
 // One CTA per SM: two producer warps walk the range and keep a ring of tiles
 // full (TMA for K and V, 128-byte rows, 128B swizzle; bulk copies for the

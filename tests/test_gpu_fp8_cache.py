@@ -244,6 +244,20 @@ def test_decode_every_group_width(cuda_lib, g):
     _check_decode(c, q, out)
 
 
+# More (row, kv head) pairs than SMs, some long enough that the split cuts
+# them: the join takes a pair's 5 to 16 q heads in one CTA.
+@pytest.mark.parametrize("Hq,Hk,rows", [(64, 8, 24), (56, 8, 24), (40, 8, 24), (24, 8, 24), (32, 2, 80),
+                                        (27, 3, 60), (24, 4, 50), (5, 1, 151)])
+@pytest.mark.parametrize("long", [900, 5000])
+def test_decode_many_split_pairs(cuda_lib, Hq, Hk, rows, long):
+    lens = [(0, 1, 130, long, long - 77, 257, 64)[i % 7] for i in range(rows)]
+    c = Cache(Hq + rows, lens, Hk, 64)
+    q = _q(Hq, rows, Hq)
+    out = _ops().paged_decode_fp8(q, *c.dev(), c.tables.to(DEV), c.lens_t(), SCALE)
+    _check_decode(c, q, out)
+    assert _deverr() == 0
+
+
 @pytest.mark.parametrize("spread,v_spread,sink", [(0.0, 0.0, False), (3.0, 0.5, False), (0.5, 12.0, False),
                                                   (0.5, 6.0, True)])
 def test_decode_row_scales_far_apart(cuda_lib, spread, v_spread, sink):
