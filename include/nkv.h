@@ -529,7 +529,9 @@ int nkv_copy_pages(const nkv_page_region* regions, int32_t num_regions, int64_t 
 /* named twice or also a source (nothing changes), or no free page (the      */
 /* target is left empty); each flags NKV_DEVERR_PAGES. A source may be named */
 /* by several forks. (-1, -1) pairs are padding (out_pages -2, no flag).     */
-/* At most 4096 forks per call.                                              */
+/* At most 4096 forks per call. Shared pages are read only: appended tokens  */
+/* never fall into one, but a compression rewrites a row's pages in place    */
+/* and must not be given a row that shares some.                             */
 int nkv_fork_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
                    int32_t block_size, int32_t* block_tables, int32_t max_blocks, int32_t num_rows,
                    int32_t* context_lens, int32_t* ref_counts, const int32_t* src_rows,

@@ -15,10 +15,10 @@
 // different heads at the same time, neighbours in memory.) The ranges are equal
 // whatever the lengths, and which tiles they hold depends on the lengths alone:
 // results are the same every time. A CTA finishes the pairs that lie inside its
-// range; of a pair that it shares with others it leaves the raw (m, l, O) in the workspace
-// (at most two: at its range's start and end), which a second kernel, launched
-// behind the first with programmatic dependence, joins in the CTAs' order. No
-// counters, so the workspace needs no content and outlives nothing.
+// range; of a pair that it shares with others it leaves the raw (m, l, O) in the
+// workspace (at most two: at its range's start and end), which a second kernel,
+// launched behind the first with programmatic dependence, joins in the CTAs'
+// order. No counters, so the workspace needs no content and outlives nothing.
 //
 // Calls of at most one (row, kv head) per SM whose time is latency are launched
 // as thread-block clusters of 1 to 8 CTAs instead, a cluster per (row, kv head):

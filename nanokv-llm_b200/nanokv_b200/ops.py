@@ -727,7 +727,8 @@ def fork_pages(caches, block_tables: torch.Tensor, context_lens: torch.Tensor,
 
     block_tables [rows, max_blocks], context_lens [rows] and ref_counts
     [num_pages] (all int32) are updated in place; caches as copy_pages, each
-    page [block_size, Hk, D] or, for exponent bytes, [Hk, block_size]. At most
+    page [block_size, Hk, D] or, for exponent bytes, [Hk, block_size]. Shared
+    pages are read only: do not compress a row while it shares some. At most
     4096 forks per call. Returns out_pages int32 [n]: the page that was taken,
     -1 if none was needed, -2 if the fork was not made (a target that is named
     twice or is a source, a row out of range, no free page: DEVERR_PAGES is
