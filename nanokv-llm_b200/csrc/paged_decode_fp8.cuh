@@ -828,7 +828,8 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   }
 
   // ---- cluster launch: the CTAs' rows are joined through distributed shared
-  // memory, in rank order, each CTA taking some of the group's heads
+  // memory, in rank order, each CTA taking some of the group's heads (eight a
+  // round: a single CTA with 9 to 16 heads takes two)
   const int rank = static_cast<int>(blockIdx.x) % csize;
   const int pair = static_cast<int>(blockIdx.x) / csize;
   if (merges == 0) {  // no tile fell to this CTA
@@ -840,8 +841,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   }
   __syncwarp();
   cluster_sync_all();
-  const int row = warp * csize + rank;
-  if (row < p.rows) {
+  for (int row = warp * csize + rank; row < p.rows; row += kDecode8Warps * csize) {
     float4 x[kDecode8MaxCluster];
     float2 ml[kDecode8MaxCluster];
     float M = NEG_INF;
