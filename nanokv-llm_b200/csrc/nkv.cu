@@ -1725,19 +1725,12 @@ size_t plan_smem(int64_t count) {
   return (3 * sizeof(uint32_t) * static_cast<size_t>((count + 31) / 32) + 15) / 16 * 16;
 }
 
+// The limit on dynamic shared memory is raised whatever the call needs: the
+// default of 48 KB counts the kernels' static arrays too.
 template <typename Params>
 int launch_plan(void (*kernel)(Params), const Params& p, size_t smem, bool* attr_set, void* stream) {
-  if (smem > 48 * 1024) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= kMaxDevices) return NKV_ERR_CUDA;
-    if (!attr_set[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           static_cast<int>(kMaxPlanSmem));
-      if (e != cudaSuccess) return cuda_status(e);
-      attr_set[dev] = true;
-    }
-  }
+  const int st = set_max_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(kMaxPlanSmem), attr_set);
+  if (st != NKV_OK) return st;
   return launch_dependent(kernel, dim3(1), dim3(nkv::kPagePlanThreads), smem,
                           static_cast<cudaStream_t>(stream), p);
 }
