@@ -526,9 +526,13 @@ int nkv_copy_pages(const nkv_page_region* regions, int32_t num_regions, int64_t 
 /* order, gets the i-th lowest); context_lens[dst] = context_lens[src], the  */
 /* table's other entries -1. out_pages[i] = that page, -1 if none was        */
 /* needed, -2 if the fork was not made: a row outside the table, a target    */
-/* named twice or also a source (nothing changes), or no free page (the      */
-/* target is left empty); each flags NKV_DEVERR_PAGES. A source may be named */
-/* by several forks. (-1, -1) pairs are padding (out_pages -2, no flag).     */
+/* named twice or also a source (nothing changes), or no free page, or a      */
+/* partial last page that is none of the cache or that nobody holds (the     */
+/* target is left empty); each flags NKV_DEVERR_PAGES. So does a full page    */
+/* that nobody holds, which is counted for the source too and shared, and    */
+/* one that is none of the cache, which the target's table lacks as well. A  */
+/* source may be named by several forks. (-1, -1) pairs are padding          */
+/* (out_pages -2, no flag).                                                  */
 /* At most 4096 forks per call. Shared pages are read only: appended tokens  */
 /* never fall into one, but a compression rewrites a row's pages in place    */
 /* and must not be given a row that shares some.                             */

@@ -68,9 +68,15 @@ __device__ __forceinline__ void page_share(const PageTables& t, const PageMove* 
   const int j = static_cast<int>(e - static_cast<int64_t>(i) * t.max_blocks);
   if (j >= moves[i].shared) return;
   const int32_t page = t.in[static_cast<int64_t>(t.src_rows[i]) * t.max_blocks + j];
-  // a page of the source that nobody holds, or none of the cache, is flagged
-  if (page < 0 || page >= t.num_pages || atomicAdd(t.ref_counts + page, 1) <= 0)
+  if (page < 0 || page >= t.num_pages) {  // no page of the cache: the branch lacks it too
     raise_error(NKV_DEVERR_PAGES);
+    return;
+  }
+  const int32_t held = atomicAdd(t.ref_counts + page, 1);
+  if (held <= 0) {  // by nobody: flagged, the source's reference too
+    raise_error(NKV_DEVERR_PAGES);
+    atomicAdd(t.ref_counts + page, 1 - held);
+  }
   t.out[static_cast<int64_t>(t.dst_rows[i]) * t.max_blocks + j] = page;
 }
 
@@ -270,6 +276,8 @@ struct PageForkParams {
 };
 
 // A fork as the planning CTA holds it in shared memory; dst = -1: not made.
+// src is the source row, then the page of its last, partial tokens. page is the
+// new page, -1: none needed, -2: none to copy from, below: not found yet.
 struct PageFork {
   int32_t src, dst, len, page;
 };
@@ -284,6 +292,7 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_fork_plan_kernel(const 
   const int words = (p.num_rows + 31) / 32;
   uint32_t *read = maps, *written = maps + words, *twice = written + words;
   PageFork* forks = reinterpret_cast<PageFork*>(maps + (3 * words + 3) / 4 * 4);
+  int32_t* tail = reinterpret_cast<int32_t*>(forks + p.n);  // a fork's partial page; by_rank later on
   for (int i = threadIdx.x; i < 3 * words; i += kPagePlanThreads) maps[i] = 0u;
   __syncthreads();
   allow_dependent_launch();
@@ -292,7 +301,8 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_fork_plan_kernel(const 
   // ---- which forks can be made: rows in range, the target named once and no source
   for (int i = threadIdx.x; i < p.n; i += kPagePlanThreads) {
     const int32_t s = p.src_rows[i], d = p.dst_rows[i];
-    forks[i] = PageFork{s, d, 0, 0};
+    forks[i] = PageFork{s, d, 0, -1};
+    tail[i] = -1;
     if (s < 0 || s >= p.num_rows || d < 0 || d >= p.num_rows) continue;
     forks[i].len = p.context_lens[s];
     atomicOr(read + (s >> 5), 1u << (s & 31));
@@ -300,6 +310,7 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_fork_plan_kernel(const 
       atomicOr(twice + (d >> 5), 1u << (d & 31));
   }
   __syncthreads();
+  bool partial = false;
   for (int i = threadIdx.x; i < p.n; i += kPagePlanThreads) {
     const PageFork f = forks[i];
     const bool skip = f.src == -1 && f.dst == -1;  // padding
@@ -308,8 +319,9 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_fork_plan_kernel(const 
     if (ok) ok = f.len >= 0 && f.len <= static_cast<int64_t>(p.max_blocks) * p.block_size;
     if (!ok && !skip) raise_error(NKV_DEVERR_PAGES);
     if (!ok) forks[i].dst = -1;
+    else if (f.len % p.block_size != 0) partial = true;
   }
-  __syncthreads();
+  const bool hands_out = __syncthreads_or(partial);  // pages, to forks with a partial one
   // ---- the targets' old pages are released: a warp per target, its entries in
   // rounds of 128 loads
   for (int i = warp; i < p.n; i += kPagePlanThreads / 32) {
@@ -332,21 +344,56 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_fork_plan_kernel(const 
       }
     }
   }
+  __syncthreads();
+  // ---- the sources' pages: one that nobody holds could be handed out below. A
+  // full one is flagged and given the source's reference; of a partial one, or one
+  // that is not there, no fork is made. (Where none is handed out the sharing finds
+  // a full one.) Enough threads a fork for its table in one round, 32 at most.
+  if (hands_out) {
+    int shift = 0;
+    while (shift < 5 && (1 << shift) < p.max_blocks) ++shift;
+    for (int i = threadIdx.x >> shift; i < p.n; i += kPagePlanThreads >> shift) {
+      const PageFork f = forks[i];
+      if (f.dst < 0) continue;
+      const int32_t* from = p.block_tables + static_cast<int64_t>(f.src) * p.max_blocks;
+      const int full = f.len / p.block_size;
+      const int used = full + (f.len > full * p.block_size ? 1 : 0);
+      for (int j = threadIdx.x & ((1 << shift) - 1); j < used; j += 1 << shift) {
+        const int32_t page = from[j];
+        const bool there = page >= 0 && page < p.num_pages;
+        const bool held = there && __ldcg(p.ref_counts + page) > 0;
+        if (j == full) {
+          if (held) tail[i] = page;
+          else forks[i].page = -2;
+        } else if (there && !held) {
+          raise_error(NKV_DEVERR_PAGES);
+          atomicMax(p.ref_counts + page, 1);
+        }
+      }
+    }
+    __syncthreads();
+  }
   // ---- rank of every fork with a partial page among those, in order
   int want = 0;
   for (int base = 0; base < p.n; base += kPagePlanThreads) {
     const int i = base + threadIdx.x;
-    const bool wants = i < p.n && forks[i].dst >= 0 && forks[i].len % p.block_size != 0;
-    const unsigned mask = __ballot_sync(0xffffffffu, wants);
+    int32_t page = i < p.n && forks[i].dst >= 0 ? forks[i].page : -2;
+    const int32_t from = page != -2 ? tail[i] : -1;
+    if (from >= 0) page = -3;
+    const unsigned mask = __ballot_sync(0xffffffffu, page == -3);
     int sum;
     const int before = want + warps_exclusive_sum(__popc(mask), warp_sums, sum);
-    if (i < p.n) forks[i].page = wants ? -3 - (before + __popc(mask & ((1u << lane) - 1u))) : -1;
+    if (page == -3) page -= before + __popc(mask & ((1u << lane) - 1u));
+    if (i < p.n) {
+      forks[i].src = from;
+      forks[i].page = page;
+    }
     want += sum;
   }
-  __syncthreads();  // and the releases
+  __syncthreads();
   // ---- the lowest free pages: rank r's page to the fork of rank r. The forks
   // with a partial page, in order, start at `by_rank` (their indices).
-  int32_t* by_rank = reinterpret_cast<int32_t*>(forks + p.n);
+  int32_t* by_rank = tail;
   for (int i = threadIdx.x; i < p.n; i += kPagePlanThreads)
     if (forks[i].page <= -3) by_rank[-3 - forks[i].page] = i;
   int found = 0;
@@ -376,9 +423,7 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_fork_plan_kernel(const 
     int32_t out = -2;
     if (f.dst >= 0) {
       const int full = f.len / p.block_size;
-      int32_t from = -1;
-      if (f.page != -1) from = p.block_tables[static_cast<int64_t>(f.src) * p.max_blocks + full];
-      const bool made = f.page == -1 || (f.page >= 0 && from >= 0 && from < p.num_pages);
+      const bool made = f.page >= -1;
       if (!made) {  // no page left, or none to copy: the target stays empty
         raise_error(NKV_DEVERR_PAGES);
       } else {
@@ -387,7 +432,7 @@ __global__ void __launch_bounds__(kPagePlanThreads) page_fork_plan_kernel(const 
         if (f.page >= 0) {
           p.ref_counts[f.page] = 1;
           p.block_tables[static_cast<int64_t>(f.dst) * p.max_blocks + full] = f.page;
-          m.src = from;
+          m.src = f.src;
           m.dst = f.page;
           m.ntok = f.len - full * p.block_size;
         }

@@ -731,8 +731,9 @@ def fork_pages(caches, block_tables: torch.Tensor, context_lens: torch.Tensor,
     pages are read only: do not compress a row while it shares some. At most
     4096 forks per call. Returns out_pages int32 [n]: the page that was taken,
     -1 if none was needed, -2 if the fork was not made (a target that is named
-    twice or is a source, a row out of range, no free page: DEVERR_PAGES is
-    set; or a (-1, -1) padding pair).
+    twice or is a source, a row out of range, no free page, a partial page that
+    is none of the cache or that nobody holds: DEVERR_PAGES is set; or a
+    (-1, -1) padding pair).
     """
     device = _one_device("fork_pages", block_tables, context_lens, ref_counts, src_rows, dst_rows,
                          out_pages, *caches)
