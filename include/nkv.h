@@ -463,11 +463,12 @@ int nkv_load_kvcache_fp8(const void* k_cache, const void* v_cache, const void* k
 /* and values are what the stored rows stand for; a length 0 writes zeros; a */
 /* length past the block table is clamped and flags                          */
 /* NKV_DEVERR_DECODE_BLOCK, as does an entry on a live token that is no      */
-/* page). g = num_q_heads / num_kv_heads in [1, 16]; batch * num_kv_heads    */
-/* <= 65536, max_blocks * block_size < 2^31 - 127, and that * batch *        */
-/* num_kv_heads <= 2^36; q and out 16-byte aligned, strides multiples of 8. The */
-/* workspace needs no particular content and nothing in it outlives the      */
-/* call: calls that may overlap on the GPU take one each.                    */
+/* page: its tokens count as zero keys and values). g = num_q_heads /        */
+/* num_kv_heads in [1, 16]; batch * num_kv_heads <= 65536, max_blocks *      */
+/* block_size < 2^31 - 127, and that * batch * num_kv_heads <= 2^36; q and   */
+/* out 16-byte aligned, strides multiples of 8. The workspace needs no       */
+/* particular content and nothing in it outlives the call: calls that may    */
+/* overlap on the GPU take one each.                                         */
 size_t nkv_paged_decode_fp8_workspace_size(int32_t num_q_heads, int32_t num_kv_heads);
 int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride_head,
                          const void* k_cache, const void* v_cache, const void* k_exp,

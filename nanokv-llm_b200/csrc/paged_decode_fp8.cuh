@@ -215,12 +215,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     *abort_flag = 0;
     fence_barrier_init();
   }
-  // exponent bytes that no copy fills (a table entry that is no page) are finite
-  for (int s = 0; s < kStages; ++s)
-    if (threadIdx.x < 16)
-      reinterpret_cast<uint4*>(smem + s * S::kStageBytes + 2 * kDecode8TileBytes + S::kQBytes)[threadIdx.x] =
-          make_uint4(0u, 0u, 0u, 0u);
-  fence_proxy_async_shared();
   if (threadIdx.x == kDecode8Warps * 32) {
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
@@ -479,7 +473,22 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         const int valid = min(kTokens, len - (t + j) * kTokens);
         const int boxes = (valid + p.box_rows - 1) >> box_shift;
         const int at = lane - first;
-        if (at >= 0 && at < boxes) {
+        const unsigned with_exps = (good >> first) & (0xffu >> (8 - boxes));
+        if (with_exps != 0xffu >> (8 - boxes)) {
+          // A box without a page: its values are filled with zeros, its exponent
+          // bytes (what the stage held last, maybe 255) here, so that its tokens
+          // count as zero keys and values. Before the stage is published.
+          ok = wait_empty();
+          if (ok && at >= 0 && at < boxes && !((good >> lane) & 1u)) {
+            for (int x = 0; x < NH * p.box_rows; x += 16)
+              *reinterpret_cast<uint4*>(smem + stage * S::kStageBytes + exp_off + x / p.box_rows * kTokens +
+                                        (at << box_shift) + x % p.box_rows) = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_shared();
+            raise_error(NKV_DEVERR_DECODE_BLOCK);
+          }
+          ok = __all_sync(0xffffffffu, ok) != 0;
+        }
+        if (ok && at >= 0 && at < boxes) {
           ok = wait_empty();
           if (ok) {
             const uint32_t sbase = smem_u32(smem + stage * S::kStageBytes);
@@ -489,7 +498,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
                 meta[stage] =
                     make_int4(b, h, seg_flags | (j == 0 ? kFirst : 0) | (j == count - 1 ? kLast : 0) | (valid << 8), 0);
               }
-              const unsigned with_exps = (good >> first) & (0xffu >> (8 - boxes));
               mbar_arrive_expect_tx(bar, (((boxes * 128u + __popc(with_exps)) * NH) << box_shift) +
                                              (j == 0 ? q_bytes : 0u));
               if (for_k && j == 0) {
@@ -511,8 +519,6 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
               for (int hh = 0; hh < NH; ++hh)
                 bulk_load_row(sbase + exp_off + hh * kTokens + (at << box_shift), exp_src + hh * p.block_size,
                               p.box_rows, bar);
-            } else {
-              raise_error(NKV_DEVERR_DECODE_BLOCK);
             }
           }
         }

@@ -1,0 +1,41 @@
+"""GPU tests of what the 8-bit decode makes of rows at the edge of its number
+formats and of table entries that name no page."""
+
+import pytest
+import torch
+
+from oracle.fp8_cache import decode_fp8_ref
+from tests.test_gpu_fp8_cache import DEV, SCALE, Cache, _deverr, _ops, _q
+
+pytestmark = pytest.mark.gpu
+
+
+def _within(c, q, out, tables, lens):
+    k, v, ke, ve = (t.to(DEV) for t in (c.k, c.v, c.ke, c.ve))
+    ref, bound = decode_fp8_ref(q, k, v, ke, ve, tables.to(DEV), lens, SCALE)
+    off = (out.double() - ref).abs()
+    assert torch.isfinite(out.float()).all()
+    assert bool((off <= bound).all()), f"{(off - bound).max().item()} over the bound"
+
+
+@pytest.mark.parametrize("Hk,g,block", [(8, 4, 64), (8, 2, 16), (7, 3, 64), (3, 16, 128), (8, 8, 32)])
+@pytest.mark.parametrize("rows", [400, 10])
+def test_an_entry_without_a_page_counts_as_zeros(cuda_lib, Hk, g, block, rows):
+    """Long rows whose tables name no page in places, behind rows of one token
+    whose pages' unused exponent bytes are 255."""
+    from nanokv_b200 import _lib
+
+    lens = [1000 if i % 10 == 9 else 1 for i in range(rows)]
+    c = Cache(Hk, lens, Hk, block, spare=1)
+    zero = next(p for p in range(c.blocks) if not bool((c.tables == p).any()))
+    c.k[zero] = c.v[zero] = 0
+    c.ke[zero] = c.ve[zero] = 127
+    bad, tables = c.tables.clone(), c.tables.clone()
+    for b in range(9, rows, 10):
+        for j, entry in ((200 // block, -1), (500 // block, c.blocks), (999 // block, -7)):
+            bad[b, j], tables[b, j] = entry, zero
+    q = _q(Hk, rows, Hk * g)
+    out = torch.full(q.shape, float("nan"), dtype=torch.bfloat16, device=DEV)
+    _ops().paged_decode_fp8(q, *c.dev(), bad.to(DEV), c.lens_t(), SCALE, out=out)
+    assert _deverr() == _lib.DEVERR_DECODE_BLOCK
+    _within(c, q, out, tables, c.lens_t())
