@@ -44,11 +44,12 @@
 //     [1, 2) and rounded to f16: 11 bits for a bf16's 8, so only elements
 //     below 2^-14 of the maximum lose any (at most 2^-25 of the maximum).
 //   * K's exponents and that power of two multiply the 32-bit scores.
-//   * V's exponents go into the weights: w_j = 2^(s_j + k_j - M) with M the
-//     running maximum of s_j + k_j (s in log2 units), so w <= 1 and what matters
-//     most has f16's full 11 bits, however far the rows' scales are apart. The
-//     softmax's own maximum m and sum l are kept beside it in 32 bits; at the
-//     end O is multiplied by 2^(M - m).
+//   * V's exponents go into the weights: w_j = 2^(s_j + k_j - M + 15) with M the
+//     running maximum of s_j + k_j (s in log2 units), so w <= 2^15 (f16 reaches
+//     65,504) and has f16's full 11 bits down to 2^-29 of the largest, however
+//     far the rows' scales are apart; below it is off by at most 2^-40 of the
+//     largest. The softmax's own maximum m and sum l are kept beside it in 32
+//     bits; at the end O is multiplied by 2^-15 and by 2^(M - m).
 // Rows of 8-bit values come out of ldmatrix as 16-bit pairs: for K two dims of
 // a token (the k order of the product is permuted to match, in q's fragments
 // too), for V, transposed, two dims of two tokens; one byte permute makes them
@@ -72,6 +73,7 @@ constexpr int kDecode8MaxCtas = 160;
 constexpr int kDecode8ORow = 132;   // floats of one row of a partial: O[128], m, l, 2 of padding
 constexpr int kDecode8JoinWarps = 16;  // at most; no fewer than the q heads of a tile
 constexpr int kDecode8MaxCluster = 8;
+constexpr int kDecode8WeightExp = 15;  // the largest weight is 2^this
 
 template <int G, int NH>
 struct Decode8Shape {
@@ -698,7 +700,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
           wx[c & 1] = fmaxf(wx[c & 1], v + vk[mt][c >> 1]);
         }
       }
-      float m_use[2], w_use[2], w_scale[2];
+      float m_use[2], w_low[2], w_scale[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -709,9 +711,10 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
         const float m_new = fmaxf(m_run[e], mx[e]);
         const float w_new = fmaxf(w_run[e], wx[e]);
         m_use[e] = m_new == NEG_INF ? 0.f : m_new;
-        w_use[e] = w_new == NEG_INF ? 0.f : w_new;
+        const float w_use = w_new == NEG_INF ? 0.f : w_new;
+        w_low[e] = w_use - kDecode8WeightExp;
         l_run[e] *= fast_exp2(m_run[e] - m_use[e]);
-        w_scale[e] = fast_exp2(w_run[e] - w_use[e]);
+        w_scale[e] = fast_exp2(w_run[e] - w_use);
         m_run[e] = m_new;
         w_run[e] = w_new;
       }
@@ -722,7 +725,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           l_run[c & 1] += fast_exp2(s[mt][c] - m_use[c & 1]);
-          w[c] = fast_exp2(s[mt][c] + vk[mt][c >> 1] - w_use[c & 1]);
+          w[c] = fast_exp2(s[mt][c] + vk[mt][c >> 1] - w_low[c & 1]);
         }
         wb[mt][0] = movmatrix_trans(pack_f16x2(w[0], w[1]));
         wb[mt][1] = movmatrix_trans(pack_f16x2(w[2], w[3]));
@@ -789,10 +792,11 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
       if (head < heads) {
         const float m = m_run[e];
         const float f = m == NEG_INF ? 0.f : fast_exp2(w_run[e] - m);
+        constexpr float kDown = 1.f / (1 << kDecode8WeightExp);
         float* dst = state + slot * S::kStateFloats + (warp * S::kWarpHeads + head) * kDecode8ORow;
 #pragma unroll
         for (int dm = 0; dm < 8; ++dm)
-          *reinterpret_cast<float2*>(dst + 16 * dm + 2 * gid) = make_float2(o[dm][e] * f, o[dm][2 + e] * f);
+          *reinterpret_cast<float2*>(dst + 16 * dm + 2 * gid) = make_float2(o[dm][e] * kDown * f, o[dm][2 + e] * kDown * f);
         if (gid == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(m, l);
       }
     }

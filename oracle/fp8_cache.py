@@ -100,10 +100,11 @@ def decode_fp8_ref(q, k_codes, v_codes, k_exp, v_exp, tables, lens, scale):
         (2^-20 + len / 16 * 2^-24) * A;
       * underflow: a weight below 2^-126 is 0 in 32 bits, which moves the
         result by at most 2^-126 |V_j| for each token; a product weight
-        w_j = p_j * 2^k_j (k_j the row's exponent) held in f16 relative to the
-        largest, W, has the absolute error 2^-25 W where it is below 2^-14 W
-        (f16's subnormal step is 2^-24), which moves the result by
-        2^-25 W |code_j| for each such token.
+        w_j = p_j * 2^k_j (k_j the row's exponent) held in f16 as 2^15 times
+        its share of the largest, W, has the absolute error 2^-40 W where it is
+        below 2^-29 W (f16's normal numbers begin at 2^-14 and its subnormal
+        step is 2^-24: half of it, over 2^15), which moves the result by
+        2^-40 W |code_j| for each such token.
     """
     B, Hq, D = q.shape
     Hk = k_codes.shape[2]
@@ -123,7 +124,7 @@ def decode_fp8_ref(q, k_codes, v_codes, k_exp, v_exp, tables, lens, scale):
             two_k = _two(byte - 127)
             w = p * two_k
             top = w.amax(-1, keepdim=True)
-            small = torch.where(w < 2.0 ** -14 * top, 2.0 ** -25 * top, 0.0)
+            small = torch.where(w < 2.0 ** -29 * top, 2.0 ** -40 * top, 0.0)
             under = small @ (v[:, h].abs() / two_k.unsqueeze(1)) + 2.0 ** -126 * v[:, h].abs().sum(0)
             e = 130 * 2.0 ** -24 * float((qq.abs() @ k[:, h].abs().T).amax()) * scale
             o = p @ v[:, h]

@@ -18,6 +18,28 @@ def _within(c, q, out, tables, lens):
     assert bool((off <= bound).all()), f"{(off - bound).max().item()} over the bound"
 
 
+@pytest.mark.parametrize("rows,Hk,g", [(4, 2, 4), (50, 2, 4), (100, 1, 12), (300, 2, 1)])
+def test_many_light_values_behind_a_heavy_one(cuda_lib, rows, Hk, g):
+    """Every warp's first token weighs 2^26 times as much as each of the others
+    (V's scales), and is zero but in dim 0: the others are the result."""
+    n = 1500
+    c = Cache(rows, [n] * rows, Hk, 128)
+    c.k.zero_()
+    c.v.fill_(0x38)  # 1.0
+    c.ke.fill_(127)
+    c.ve.fill_(127 - 13)
+    pages = c.tables.long()
+    for t in range(0, 256, 32):
+        at = pages[:, t // 128]
+        c.v[at, t % 128, :, 1:] = 0
+        c.ve[at, :, t % 128] = 127 + 13
+    q = _q(rows, rows, Hk * g)
+    out = torch.full(q.shape, float("nan"), dtype=torch.bfloat16, device=DEV)
+    _ops().paged_decode_fp8(q, *c.dev(), c.tables.to(DEV), c.lens_t(), SCALE, out=out)
+    _within(c, q, out, c.tables, c.lens_t())
+    assert _deverr() == 0
+
+
 @pytest.mark.parametrize("Hk,g,block", [(8, 4, 64), (8, 2, 16), (7, 3, 64), (3, 16, 128), (8, 8, 32)])
 @pytest.mark.parametrize("rows", [400, 10])
 def test_an_entry_without_a_page_counts_as_zeros(cuda_lib, Hk, g, block, rows):
