@@ -488,7 +488,8 @@ int nkv_paged_decode_fp8(const void* q, int64_t q_stride_token, int64_t q_stride
 /* <= 0 = free). Every decision is taken on the device, so the calls can be  */
 /* captured in a CUDA graph; free pages are taken lowest first. Tables and   */
 /* counts named by a call must not be changed by another one that may        */
-/* overlap with it.                                                          */
+/* overlap with it. An nkv_decode_step behind one of these calls takes       */
+/* metadata_ready = 0 unless host copies of its metadata lie between them.   */
 
 /* One cache tensor (host struct): `lead` copies (layers, K and V) of        */
 /* num_pages contiguous pages, lead_stride bytes apart. A page is page_bytes */

@@ -108,4 +108,5 @@ class StepMetadata:
         set_context(all_decode, cu_q, cu_k, self.max_seqlen_q, self.max_seqlen_k, slot_mapping,
                     context_lens, block_tables)
         get_context().total_seqlen_k = int(self.cu_seqlens_k[-1])
+        get_context().metadata_from_host = True
         return input_ids, positions, logits_indices

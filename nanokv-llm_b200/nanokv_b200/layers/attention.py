@@ -30,7 +30,7 @@ from torch import nn
 
 from .. import ops
 from ..ops import store_kvcache  # noqa: F401  (same public name as the reference module)
-from ..utils.context import get_context
+from ..utils.context import get_context, metadata_ready
 from .compress_utils import MyCompressCompact
 
 
@@ -113,11 +113,11 @@ class Attention(nn.Module):
         if (not stored and context.use_decode_kernel and not compressing and k_cache.numel()
                 and q.size(0) == context.block_tables.size(0)):
             # decode step without compression: slot write + decode in one launch;
-            # the step's metadata comes from host copies, so no kernel right
+            # where the step's metadata comes from host copies, no kernel right
             # before this one writes it
             o = ops.decode_step(q, k, v, k_cache, v_cache, context.slot_mapping,
                                 context.block_tables, context.context_lens, self.scale,
-                                metadata_ready=True)
+                                metadata_ready=metadata_ready(context))
             return o.unsqueeze(1)
         if not stored and k_cache.numel() and v_cache.numel():
             ops.store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)

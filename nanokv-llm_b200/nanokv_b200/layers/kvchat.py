@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from .. import ops
-from ..utils.context import get_context
+from ..utils.context import get_context, metadata_ready
 
 
 def MyCompressCompact(query_window_manager, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -126,10 +126,10 @@ class Attention(nn.Module):
                 ring_args = dict(ring=qwm.ring, layer_id=Layer,
                                  ring_slot_of_row=context.q_window_row_slot_t,
                                  ring_pos_of_row=context.q_window_row_pos_t)
-            # the step's metadata and ring indices come from host copies
+            # ring indices come from host copies, and as a rule the step's metadata
             o = ops.decode_step(q, k, v, k_cache, v_cache, context.slot_mapping,
                                 context.block_tables, context.context_lens, self.scale,
-                                metadata_ready=True, **ring_args)
+                                metadata_ready=metadata_ready(context), **ring_args)
             if ring_args:
                 qwm.advance(context.q_window_active_seq_ids, Layer)
             return o.unsqueeze(1)

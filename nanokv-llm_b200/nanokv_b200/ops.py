@@ -17,6 +17,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
+from .utils.context import note_page_call
 
 __all__ = [
     "store_kvcache",
@@ -178,7 +179,8 @@ def decode_step(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_cache
     slot_mapping or the ring indices (host copies and earlier kernels are
     fine), so the launch may read them before it waits for that kernel --
     true of a decode step's layers, whose metadata the engine copies from
-    the host; not of a decode right after a compression kernel."""
+    the host; not of a decode right after a compression kernel or a page
+    operator (copy_pages, fork_pages, free_pages, compact_pages)."""
     _require_cuda("decode_step", q, key, value, k_cache, v_cache, slot_mapping, block_tables,
                   context_lens)
     B, Hq, D = q.shape
@@ -712,6 +714,7 @@ def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor, page_dim: int = 0) 
     if n == 0 or count == 0:
         return
     ws, size = _pages_workspace(src, n, 0)
+    note_page_call()
     _call(device, "nkv_copy_pages", regions, count, num_pages, src.data_ptr(), dst.data_ptr(), n,
           ws.data_ptr(), size)
 
@@ -747,6 +750,7 @@ def fork_pages(caches, block_tables: torch.Tensor, context_lens: torch.Tensor,
     if n == 0:
         return out_pages
     ws, size = _pages_workspace(src_rows, n, 0)
+    note_page_call()
     _call(device, "nkv_fork_pages", regions, count, num_pages, block_size,
           block_tables.data_ptr(), max_blocks, rows, context_lens.data_ptr(),
           ref_counts.data_ptr(), src_rows.data_ptr(), dst_rows.data_ptr(), n,
@@ -766,6 +770,7 @@ def free_pages(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_count
     assert context_lens.numel() == num_rows
     if n == 0:
         return
+    note_page_call()
     _call(device, "nkv_free_pages", block_tables.data_ptr(), max_blocks, num_rows,
           context_lens.data_ptr(), ref_counts.data_ptr(), ref_counts.numel(), block_size,
           rows.data_ptr(), n, 1 if trim else 0)
@@ -794,6 +799,7 @@ def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, 
     assert out_ref_counts.numel() == num_pages and out_num_live.numel() == 1
     _keep, regions, count, _ = _page_regions(caches, page_dim, num_pages, None)
     ws, size = _pages_workspace(ref_counts, num_pages // 2, num_pages)
+    note_page_call()
     _call(device, "nkv_compact_pages", regions, count, num_pages, block_tables.data_ptr(),
           out_block_tables.data_ptr(), rows * max_blocks, ref_counts.data_ptr(),
           out_ref_counts.data_ptr(), out_num_live.data_ptr(), ws.data_ptr(), size)

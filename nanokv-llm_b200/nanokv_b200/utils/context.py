@@ -24,6 +24,15 @@ Additions, all optional and defaulting to "not provided":
                              compression step then frees the pages that its
                              rows no longer reach on the device
                              (ops.free_pages), block_tables included
+  metadata_from_host         whether the decode layers may vouch for the step's
+                             metadata (ops.decode_step, metadata_ready). True:
+                             block_tables, context_lens and slot_mapping reached
+                             the device by host copies and no page operator
+                             (ops.copy_pages, fork_pages, free_pages,
+                             compact_pages) was called since;
+                             StepMetadata.set_context sets it. The page operators
+                             set it to False. None (not provided): True as long
+                             as this process has called none of them
   compress_device_select, compress_topk, compress_tail_uncompressed_t,
   compress_selected_host     selection of a periodic compression step on the
                              device, so the step can be replayed from a CUDA
@@ -78,6 +87,7 @@ class Context:
 
     total_seqlen_k: int = 0
     page_ref_counts: torch.Tensor | None = None
+    metadata_from_host: bool | None = None
 
     # device-side selection of a periodic compression step (graph-capturable):
     # the layers select at layer 0 into compress_selected_t ([topk], -1
@@ -91,6 +101,22 @@ class Context:
 
 
 _CONTEXT = Context()
+_PAGES_CALLED = False  # a page operator, in this process
+
+
+def note_page_call() -> None:
+    """A page operator is about to write tables, lengths or cache rows on the
+    device: the layers of the current step, and of later ones whose metadata is
+    not known to come from the host, wait for the kernel ahead of them."""
+    global _PAGES_CALLED
+    _PAGES_CALLED = True
+    _CONTEXT.metadata_from_host = False
+
+
+def metadata_ready(context: Context) -> bool:
+    """Whether a decode layer may vouch for the step's metadata."""
+    known = context.metadata_from_host
+    return not _PAGES_CALLED if known is None else known
 
 
 def get_context() -> Context:

@@ -1,0 +1,101 @@
+"""What the layers vouch for before and after the page operators, which write
+tables, lengths and cache rows on the device. Host logic only: no GPU."""
+
+import types
+
+import numpy as np
+import pytest
+import torch
+
+I32 = torch.int32
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """ops with the launches taken out; the metadata_ready of every decode step."""
+    from nanokv_b200 import build, ops
+    from nanokv_b200.utils import context
+
+    build.build()
+    seen = []
+
+    def decode_step(q, *args, metadata_ready=False, **kw):
+        seen.append(metadata_ready)
+        return q
+
+    monkeypatch.setattr(ops, "decode_step", decode_step)
+    monkeypatch.setattr(ops, "_one_device", lambda *a: 0)
+    monkeypatch.setattr(ops, "_call", lambda *a: None)
+    monkeypatch.setattr(context, "_PAGES_CALLED", False, raising=False)
+    yield seen
+    context.reset_context()
+
+
+def _layer(kind):
+    from nanokv_b200.layers import attention, kvchat
+
+    cfg = types.SimpleNamespace(kv_compress_enabled=False, kv_compress_N=4, kv_compress_S=9, kv_compress_R=5)
+    module = {"periodic": attention, "threshold": kvchat}[kind]
+    a = module.Attention(4, 128, 0.1, 2, cfg, 1)
+    a.k_cache = a.v_cache = torch.zeros(2, 16, 2, 128, dtype=torch.bfloat16)
+    return a
+
+
+def _forward(a):
+    a.forward(torch.zeros(2, 4, 128), torch.zeros(2, 2, 128), torch.zeros(2, 2, 128), 0)
+
+
+def _page_calls():
+    from nanokv_b200 import ops
+
+    cache = torch.zeros(2, 16, 2, 128, dtype=torch.bfloat16)
+    t, n, r = torch.zeros(2, 1, dtype=I32), torch.zeros(2, dtype=I32), torch.ones(2, dtype=I32)
+    return {"copy": lambda: ops.copy_pages([cache], n, n), "fork": lambda: ops.fork_pages([cache], t, n, r, n, n, 16),
+            "free": lambda: ops.free_pages(t, n, r, n, 16), "compact": lambda: ops.compact_pages([cache], t, r)}
+
+
+def _set_context():
+    from nanokv_b200.utils.context import set_context
+
+    set_context(True, slot_mapping=torch.zeros(2, dtype=I32), context_lens=torch.ones(2, dtype=I32),
+                block_tables=torch.zeros(2, 1, dtype=I32))
+
+
+def _upload():
+    from nanokv_b200.engine.step_metadata import StepMetadata
+
+    one, two = np.ones(2, dtype=np.int32), np.arange(3, dtype=np.int32)
+    StepMetadata(input_ids=one, positions=one, cu_seqlens_q=two, cu_seqlens_k=two, max_seqlen_q=1,
+                 max_seqlen_k=1, slot_mapping=one, context_lens=one, logits_indices=one,
+                 block_tables=one.reshape(2, 1)).set_context(True, "cpu", pin=False)
+
+
+@pytest.mark.parametrize("kind", ["periodic", "threshold"])
+@pytest.mark.parametrize("name", ["copy", "fork", "free", "compact"])
+def test_a_step_behind_a_page_call_does_not_vouch(calls, kind, name):
+    a, page = _layer(kind), _page_calls()[name]
+    _set_context()
+    _forward(a)  # no page operator so far: as ever
+    page()
+    _forward(a)  # the same Context
+    _set_context()
+    _forward(a)  # a new one whose tensors may be the ones that the call wrote
+    _upload()
+    _forward(a)  # copied from the host after the call
+    page()
+    _forward(a)
+    assert calls == [True, False, False, True, False]
+
+
+def test_an_engine_may_say_where_its_metadata_comes_from(calls):
+    from nanokv_b200.utils.context import get_context
+
+    a, page = _layer("periodic"), _page_calls()["fork"]
+    page()
+    _set_context()
+    get_context().metadata_from_host = True
+    _forward(a)
+    _set_context()
+    get_context().metadata_from_host = False
+    _forward(a)
+    assert calls == [True, False]
