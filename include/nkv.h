@@ -374,7 +374,8 @@ int nkv_query_window_append(const void* q, int64_t q_stride_token,
 /* ring queries of ring slot ring_slot_of_selected[i] (all heads, all W      */
 /* queries); SnapKV keeps token 0, the top R-W-1 and the last W; kept rows   */
 /* are compacted to positions [0, R) of the sequence's block table and       */
-/* context_lens[b] = R. out_keep_idx is optional ([num_selected, R]), and so */
+/* context_lens[b] = R. Entries of selected_batch_indices equal to -1 are    */
+/* skipped. out_keep_idx is optional ([num_selected, R]), and so             */
 /* is out_importance (bf16 [num_selected, S - W]: the importance ranked).    */
 int nkv_threshold_compress(const void* ring, int32_t num_ring_slots, int32_t num_layers,
                            int32_t window_size, int32_t layer_id,
@@ -537,7 +538,7 @@ int nkv_copy_pages(const nkv_page_region* regions, int32_t num_regions, int64_t 
 /* (out_pages -2, no flag).                                                  */
 /* At most 4096 forks per call. Shared pages are read only: appended tokens  */
 /* never fall into one, but a compression rewrites a row's pages in place    */
-/* and must not be given a row that shares some.                             */
+/* and must not be given a row that shares some (nkv_unshared_rows).         */
 int nkv_fork_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
                    int32_t block_size, int32_t* block_tables, int32_t max_blocks, int32_t num_rows,
                    int32_t* context_lens, int32_t* ref_counts, const int32_t* src_rows,
@@ -553,6 +554,17 @@ int nkv_free_pages(int32_t* block_tables, int32_t max_blocks, int32_t num_rows,
                    int32_t* context_lens, int32_t* ref_counts, int64_t num_pages,
                    int32_t block_size, const int32_t* rows, int32_t n, int32_t trim,
                    void* stream);
+
+/* out_rows[i] = rows[i] if that row may be rewritten in place, else -1: one */
+/* of the pages that a compression rewrites has more than one reference      */
+/* (flags NKV_DEVERR_PAGES), or the row is outside the table (flagged too);  */
+/* -1 stays -1. Those pages are entries [first, first + pages) of its table, */
+/* first = lens[row] / block_size - window_blocks, or 0 where lens is NULL:  */
+/* pages = the kept tokens' pages. out_rows may be rows.                     */
+int nkv_unshared_rows(const int32_t* rows, int32_t n, const int32_t* block_tables,
+                      int32_t max_blocks, int32_t num_rows, const int32_t* lens,
+                      const int32_t* ref_counts, int64_t num_pages, int32_t block_size,
+                      int32_t window_blocks, int32_t pages, int32_t* out_rows, void* stream);
 
 /* Brings the n pages in use to [0, n): the i-th page in use at or past n    */
 /* moves to the i-th free page before n (both counted upwards) in every      */

@@ -483,6 +483,45 @@ __global__ void __launch_bounds__(256) page_free_kernel(const PageFreeParams p) 
   if (!p.trim && threadIdx.x == 0) p.context_lens[row] = 0;
 }
 
+// ---------------------------------------------------------------- shared rows
+struct PageSharedParams {
+  const int32_t* rows;
+  int32_t* out_rows;  // may be rows
+  int n;
+  const int32_t* block_tables;
+  int max_blocks;
+  int num_rows;
+  const int32_t* lens;  // null: the pages are a row's first
+  const int32_t* ref_counts;
+  int64_t num_pages;
+  int block_size;
+  int window_blocks;
+  int pages;
+};
+
+// A warp per named row: which of them may be rewritten in place.
+__global__ void __launch_bounds__(32) page_shared_kernel(const PageSharedParams p) {
+  const int i = blockIdx.x, lane = threadIdx.x;
+  int32_t row = p.rows[i];
+  if (row != -1 && (row < 0 || row >= p.num_rows)) {
+    if (lane == 0) raise_error(NKV_DEVERR_PAGES);
+    row = -1;
+  }
+  if (row >= 0) {
+    const int first = p.lens != nullptr ? p.lens[row] / p.block_size - p.window_blocks : 0;
+    bool shared = false;
+    for (int j = max(first, 0) + lane; j < min(first + p.pages, p.max_blocks); j += 32) {
+      const int32_t page = p.block_tables[static_cast<int64_t>(row) * p.max_blocks + j];
+      if (page >= 0 && page < p.num_pages && p.ref_counts[page] > 1) shared = true;
+    }
+    if (__any_sync(0xffffffffu, shared)) {
+      if (lane == 0) raise_error(NKV_DEVERR_PAGES);
+      row = -1;
+    }
+  }
+  if (lane == 0) p.out_rows[i] = row;
+}
+
 // ---------------------------------------------------------------- compact plan
 struct PageCompactParams {
   const int32_t* ref_counts;

@@ -1838,6 +1838,34 @@ int nkv_free_pages(int32_t* block_tables, int32_t max_blocks, int32_t num_rows,
                           static_cast<cudaStream_t>(stream), p);
 }
 
+int nkv_unshared_rows(const int32_t* rows, int32_t n, const int32_t* block_tables,
+                      int32_t max_blocks, int32_t num_rows, const int32_t* lens,
+                      const int32_t* ref_counts, int64_t num_pages, int32_t block_size,
+                      int32_t window_blocks, int32_t pages, int32_t* out_rows, void* stream) {
+  if (n < 0 || num_pages < 0 || block_size <= 0 || max_blocks < 0 || num_rows < 0 ||
+      window_blocks < 0 || pages < 0)
+    return NKV_ERR_INVALID_ARGUMENT;
+  if (n == 0) return NKV_OK;
+  if (!rows || !out_rows || !ref_counts || (!block_tables && max_blocks > 0))
+    return NKV_ERR_INVALID_ARGUMENT;
+  if (pages > max_blocks) return NKV_ERR_INVALID_ARGUMENT;
+  nkv::PageSharedParams p{};
+  p.rows = rows;
+  p.out_rows = out_rows;
+  p.n = n;
+  p.block_tables = block_tables;
+  p.max_blocks = max_blocks;
+  p.num_rows = num_rows;
+  p.lens = lens;
+  p.ref_counts = ref_counts;
+  p.num_pages = num_pages;
+  p.block_size = block_size;
+  p.window_blocks = window_blocks;
+  p.pages = pages;
+  nkv::page_shared_kernel<<<n, 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return launch_status();
+}
+
 int nkv_compact_pages(const nkv_page_region* regions, int32_t num_regions, int64_t num_pages,
                       const int32_t* block_tables, int32_t* out_block_tables, int64_t num_entries,
                       const int32_t* ref_counts, int32_t* out_ref_counts, int32_t* out_num_live,

@@ -182,6 +182,9 @@ threshold_compress_kernel(const ThresholdCompressParams p) {
     return;
   }
   const int b = __ldg(p.selected + sel_i);
+  // -1: an entry that was taken out of the selection; uniform across the
+  // cluster, before any cluster barrier
+  if (b < 0) return;
   const int64_t bt_row = static_cast<int64_t>(b) * p.max_blocks;
   auto slot_of = [&](int pos) -> int64_t {
     const int bi = pos / bs;

@@ -141,6 +141,11 @@ SIGNATURES: dict[str, tuple] = {
         c_int,
         [_I32P, c_int32, c_int32, _I32P, _I32P, c_int64, c_int32, _I32P, c_int32, c_int32, _P],
     ),
+    "nkv_unshared_rows": (
+        c_int,
+        [_I32P, c_int32, _I32P, c_int32, c_int32, _I32P, _I32P, c_int64, c_int32, c_int32, c_int32,
+         _I32P, _P],
+    ),
     "nkv_compact_pages": (
         c_int,
         [_P, c_int32, c_int64, _I32P, _I32P, c_int64, _I32P, _I32P, _I32P, _P, c_size_t, _P],

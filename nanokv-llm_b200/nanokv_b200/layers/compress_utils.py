@@ -34,6 +34,29 @@ def _free_pages(context, selected: torch.Tensor, block_size: int) -> None:
                        selected, block_size, trim=True)
 
 
+def unshared_selection(context, selected: torch.Tensor, layer_id: int, block_size: int,
+                       kept_tokens: int, lens=None, window_blocks: int = 0) -> torch.Tensor:
+    """The selected rows of a compression step without those that would rewrite
+    a page they share with another row (a fork), which would change that row
+    too: they are -1 and flagged, the same in every layer. Known only where the
+    Context carries the pages' reference counts."""
+    if context.page_ref_counts is None:
+        return selected
+    if layer_id == 0 or context.compress_unshared_t is None:
+        context.compress_unshared_t = ops.unshared_rows(
+            selected, context.block_tables, context.page_ref_counts, block_size, kept_tokens,
+            lens=lens, window_blocks=window_blocks)
+    return context.compress_unshared_t
+
+
+def compressed_rows(context, rows: list, selected: torch.Tensor) -> list:
+    """The rows of a host-selected step that were compressed, for its events:
+    read back where some may have been left out (a capture records the host's)."""
+    if context.page_ref_counts is None or torch.cuda.is_current_stream_capturing():
+        return rows
+    return [b for b in selected.tolist() if b >= 0]
+
+
 def MyCompressCompact(q_current: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       layer_id: int, block_size: int, window_blocks: int, keep_blocks: int,
                       keep_extra_tokens: int, num_layers: int, context=None) -> bool:
@@ -67,7 +90,8 @@ def MyCompressCompact(q_current: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     if base_h is not None:
         full = [base_h[b] // B for b in selected]
         assert all(f >= window_blocks for f in full), f"some full_blocks < window_blocks: {full}"
-    sel = _selected_tensor(context, k_cache.device)
+    sel = unshared_selection(context, _selected_tensor(context, k_cache.device), layer_id, B,
+                             keep_tokens, lens=base, window_blocks=window_blocks)
     ops.window_compress(q_current, k_cache, v_cache, context.block_tables, base,
                         context.context_lens, sel, window_blocks, keep_tokens, obs_window=1)
 
@@ -79,7 +103,7 @@ def MyCompressCompact(q_current: torch.Tensor, k_cache: torch.Tensor, v_cache: t
         tables = context.block_tables_host
         if tables is None:
             tables = context.block_tables.tolist()
-        for b in selected:
+        for b in compressed_rows(context, selected, sel):
             new_len = int(base_h[b]) - window_tokens + keep_tokens
             keep_blocks_after = (new_len + B - 1) // B
             freed = [int(x) for x in tables[b][keep_blocks_after:] if int(x) >= 0]
@@ -119,6 +143,8 @@ def _compress_device_selected(q_current, k_cache, v_cache, layer_id, block_size,
         ops.window_select(context.context_lens, context.compress_tail_uncompressed_t, B,
                           window_blocks, context.compress_topk, out_selected=sel,
                           out_base_lens=base)
+    sel = unshared_selection(context, sel, layer_id, B, keep_tokens, lens=base,
+                             window_blocks=window_blocks)
     ops.window_compress(q_current, k_cache, v_cache, context.block_tables, base,
                         context.context_lens, sel, window_blocks, keep_tokens, obs_window=1)
     if layer_id + 1 >= num_layers:

@@ -17,6 +17,7 @@ from torch import nn
 
 from .. import ops
 from ..utils.context import get_context, metadata_ready
+from .compress_utils import compressed_rows, unshared_selection
 
 
 def MyCompressCompact(query_window_manager, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -45,6 +46,7 @@ def MyCompressCompact(query_window_manager, k_cache: torch.Tensor, v_cache: torc
                          dtype=torch.int32).to(dev, non_blocking=True)
         sel, slots = t[0], t[1]
         context.compress_selected_t, context.compress_ring_slots_t = sel, slots
+    sel = unshared_selection(context, sel, layer_id, block_size, R)
     ops.threshold_compress(query_window_manager.ring, slots, layer_id, k_cache, v_cache,
                            context.block_tables, context.context_lens, sel, S, R)
     if layer_id + 1 >= num_layers:
@@ -54,7 +56,7 @@ def MyCompressCompact(query_window_manager, k_cache: torch.Tensor, v_cache: torc
             tables = context.block_tables.tolist()
         if context.compression_events is None:
             context.compression_events = []
-        for b in seq_idxs:
+        for b in compressed_rows(context, seq_idxs, sel):
             context.compression_events.append({
                 "batch_index": int(b),
                 "layer": int(layer_id),

@@ -38,6 +38,7 @@ __all__ = [
     "copy_pages",
     "fork_pages",
     "free_pages",
+    "unshared_rows",
     "compact_pages",
 ]
 
@@ -731,7 +732,8 @@ def fork_pages(caches, block_tables: torch.Tensor, context_lens: torch.Tensor,
     block_tables [rows, max_blocks], context_lens [rows] and ref_counts
     [num_pages] (all int32) are updated in place; caches as copy_pages, each
     page [block_size, Hk, D] or, for exponent bytes, [Hk, block_size]. Shared
-    pages are read only: do not compress a row while it shares some. At most
+    pages are read only: do not compress a row while it shares some
+    (unshared_rows). At most
     4096 forks per call. Returns out_pages int32 [n]: the page that was taken,
     -1 if none was needed, -2 if the fork was not made (a target that is named
     twice or is a source, a row out of range, no free page, a partial page that
@@ -774,6 +776,31 @@ def free_pages(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_count
     _call(device, "nkv_free_pages", block_tables.data_ptr(), max_blocks, num_rows,
           context_lens.data_ptr(), ref_counts.data_ptr(), ref_counts.numel(), block_size,
           rows.data_ptr(), n, 1 if trim else 0)
+
+
+def unshared_rows(rows: torch.Tensor, block_tables: torch.Tensor, ref_counts: torch.Tensor,
+                  block_size: int, kept_tokens: int, lens: torch.Tensor | None = None,
+                  window_blocks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The named rows (int32 on the device, -1 stays) that a compression may
+    rewrite in place: one that shares a page which the compression would write
+    (the kept tokens' pages, from the window's first page on or, without lens,
+    from the row's first) becomes -1 and sets DEVERR_PAGES."""
+    device = _one_device("unshared_rows", rows, block_tables, ref_counts, lens, out)
+    if out is None:
+        out = torch.empty_like(rows, memory_format=torch.contiguous_format)
+    num_rows, max_blocks = _check_page_state(block_tables, rows, ref_counts, out)
+    n = rows.numel()
+    assert out.numel() == n
+    if lens is not None:
+        assert lens.dtype is _INT32 and lens.is_contiguous()
+        num_rows = min(num_rows, lens.numel())
+    if n == 0:
+        return out
+    pages = min(-(-kept_tokens // block_size), max_blocks)
+    _call(device, "nkv_unshared_rows", rows.data_ptr(), n, block_tables.data_ptr(), max_blocks,
+          num_rows, _ptr(lens), ref_counts.data_ptr(), ref_counts.numel(), block_size,
+          window_blocks, pages, out.data_ptr())
+    return out
 
 
 def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, page_dim: int = 0,

@@ -23,7 +23,10 @@ Additions, all optional and defaulting to "not provided":
   page_ref_counts            int32 [num_pages] device tensor: a periodic
                              compression step then frees the pages that its
                              rows no longer reach on the device
-                             (ops.free_pages), block_tables included
+                             (ops.free_pages), block_tables included; and any
+                             compression leaves rows as they are that would
+                             rewrite a page they share (ops.unshared_rows, into
+                             compress_unshared_t)
   metadata_from_host         whether the decode layers may vouch for the step's
                              metadata (ops.decode_step, metadata_ready). True:
                              block_tables, context_lens and slot_mapping reached
@@ -87,6 +90,7 @@ class Context:
 
     total_seqlen_k: int = 0
     page_ref_counts: torch.Tensor | None = None
+    compress_unshared_t: torch.Tensor | None = None
     metadata_from_host: bool | None = None
 
     # device-side selection of a periodic compression step (graph-capturable):

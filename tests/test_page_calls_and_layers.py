@@ -99,3 +99,17 @@ def test_an_engine_may_say_where_its_metadata_comes_from(calls):
     get_context().metadata_from_host = False
     _forward(a)
     assert calls == [True, False]
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(n=0), 0), (dict(n=-1), 1), (dict(rows=None), 1), (dict(out=None), 1), (dict(refs=None), 1),
+    (dict(tables=None), 1), (dict(block=0), 1), (dict(mb=-1), 1), (dict(window=-1), 1), (dict(pages=-1), 1),
+    (dict(pages=5), 1), (dict(num_rows=-1), 1), (dict(num_pages=-1), 1)])
+def test_unshared_rows_refusals(kw, status):
+    from nanokv_b200 import _lib, build
+
+    build.build()
+    a = dict(rows=16, n=1, tables=16, mb=4, num_rows=2, lens=16, refs=16, num_pages=8, block=16, window=2, pages=1,
+             out=16)
+    a.update(kw)
+    assert _lib.load().nkv_unshared_rows(*a.values(), None) == status
