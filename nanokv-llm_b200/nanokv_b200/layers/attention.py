@@ -20,7 +20,8 @@ With an 8-bit cache (k_cache / v_cache float8_e4m3fn, and k_exp / v_exp, their
 exponent bytes, set beside them) the rows are stored by nkv_store_kvcache_fp8
 and decode is nkv_paged_decode_fp8; a prompt chunk over a cached prefix reads
 its sequences back in bf16 (nkv_load_kvcache_fp8) and attends over them. The
-compressions work on a bf16 cache only and are refused.
+compressions work on a bf16 cache only: a layer with kv_compress_enabled refuses
+an 8-bit one at its first step, before anything is stored.
 """
 
 from __future__ import annotations
@@ -87,8 +88,8 @@ class Attention(nn.Module):
     def _attend_fp8(self, q, k, v):
         context = get_context()
         cache = (self.k_cache, self.v_cache, self.k_exp, self.v_exp)
-        if self.kv_compress_enabled and context.is_compress_step:
-            raise ValueError("KV compression needs a bf16 cache")
+        if self.kv_compress_enabled:  # at the first step, not at the first that compresses
+            raise ValueError("KV compression (kv_compress_enabled) needs a bf16 cache")
         if self.k_cache.numel():
             ops.store_kvcache_fp8(k, v, *cache, context.slot_mapping)
         if context.use_decode_kernel:

@@ -113,3 +113,39 @@ def test_unshared_rows_refusals(kw, status):
              out=16)
     a.update(kw)
     assert _lib.load().nkv_unshared_rows(*a.values(), None) == status
+
+
+@pytest.mark.parametrize("decode", [False, True])
+@pytest.mark.parametrize("entry", ["forward", "forward_qkv"])
+def test_compression_of_an_8_bit_cache_is_refused_at_the_first_step(calls, monkeypatch, decode, entry):
+    """Whatever the step is: not in the middle of serving, at the first that compresses."""
+    from nanokv_b200 import ops
+    from nanokv_b200.layers.attention import Attention
+    from nanokv_b200.utils.context import set_context
+
+    stored = []
+    monkeypatch.setattr(ops, "store_kvcache_fp8", lambda *a: stored.append(a))
+    monkeypatch.setattr(ops, "paged_decode_fp8", lambda q, *a: q)
+    monkeypatch.setattr(ops, "flash_attn_varlen_func", lambda q, *a, **kw: q)
+    q, k = torch.zeros(2, 4, 128), torch.zeros(2, 2, 128)
+    monkeypatch.setattr(ops, "qk_norm_rope_store", lambda *a, **kw: (q, k, k))
+    for enabled in (False, True):
+        cfg = types.SimpleNamespace(kv_compress_enabled=enabled, kv_compress_window_blocks=4,
+                                    kv_compress_keep_blocks=2, kv_compress_keep_extra_tokens=1)
+        a = Attention(4, 128, 0.1, 2, cfg, 1)
+        a.k_cache = a.v_cache = torch.zeros(2, 16, 2, 128, dtype=torch.uint8).view(torch.float8_e4m3fn)
+        a.k_exp = a.v_exp = torch.zeros(2, 2, 16, dtype=torch.uint8)
+        i = torch.zeros(2, dtype=I32)
+        set_context(decode, i, i, 1, 1, i, i, None)
+
+        def run():
+            if entry == "forward":
+                return a.forward(q, k, k, 0)
+            return a.forward_qkv(torch.zeros(2, 8 * 128), i, None, None, None, 1e-6, 0)
+
+        if enabled:
+            with pytest.raises(ValueError, match="needs a bf16 cache"):
+                run()
+            assert len(stored) == 1
+        else:
+            run()
