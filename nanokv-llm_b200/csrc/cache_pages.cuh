@@ -90,7 +90,8 @@ __device__ __forceinline__ void page_remap(const PageTables& t, int64_t e) {
   t.out[e] = page;
 }
 
-// Bound by HBM: each page is read and written once. A CTA takes items of 64 KB,
+// Bound by HBM: each move reads a page and writes one (a partial page that several
+// branches get is read for each, partly from L2). A CTA takes items of 64 KB,
 // every thread sixteen 16-byte loads and then their stores, so that a CTA has
 // 64 KB in flight. (Bulk copies through shared memory measured the same or
 // slower but for many forks: 21 pages of 28 layers 200 us each way, a pool of

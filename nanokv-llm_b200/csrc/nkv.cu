@@ -1345,9 +1345,11 @@ int encode_cache8(CUtensorMap* map, const void* base, int num_kv_heads, int64_t 
 // before the two launches of the split form, and a CTA of it has T / C tiles
 // instead of P T / SMs: it is taken while that is at most 5 tiles more (one row
 // x 8 heads: 8,192 tokens 10.1 against 10.3 us, 16,384 15.6 against 13.0; x 1
-// head: 4,096 7.5 against 7.9, 8,192 10.0 against 8.6; 4 rows x 8: 8,192 16.5
-// against 18.9). And up to 12 tiles a CTA, because T comes from the table's
-// width: the split balances rows that are shorter.
+// head: 4,096 7.5 against 7.9, 8,192 10.0 against 8.6). And up to 12 tiles a CTA,
+// because T comes from the table's width: the split balances rows that are
+// shorter. (Rows as long as their table pay for that cap: 4 rows x 8 heads of
+// 8,192 tokens, 16 tiles a CTA, take 18.9 in the split and would take 16.5.)
+// Where fewer clusters fit at once than pairs, smaller ones are taken.
 constexpr int kDecode8ClusterTiles = 12;
 constexpr int kDecode8ClusterMore = 5;
 
