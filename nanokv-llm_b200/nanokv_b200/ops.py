@@ -599,7 +599,8 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
     q: [B, Hq, 128] bf16 (row and head strides multiples of 8); the cache as
     store_kvcache_fp8 writes it; block_tables [B, max_blocks] int32;
-    context_lens [B] int32 (0 gives zeros). workspace (uint8, at least
+    context_lens [B] int32 (0 gives zeros; tokens whose table entry is no page
+    count as zero keys and values, DEVERR_DECODE_BLOCK is set). workspace (uint8, at least
     decode_fp8_workspace_bytes) may hold anything; by default every call takes
     its own from torch's allocator, so calls on several streams and captured
     graphs share none. Returns out [B, Hq, 128] bf16.
